@@ -338,6 +338,89 @@ int sph_kv_cache_update_into(const void* src, int src_dtype, const void* cache, 
                              int64_t n_kv, int64_t seq, int64_t head_dim, int64_t max_seq, int64_t cur_len,
                              int64_t* new_len, void* stream);
 
+/* ─────────────────────────── paged KV cache ───────────────────────────
+ * A serving batch's cache: pools kcache / vcache [n_pages, n_kv_heads,
+ * page_size, head_dim] shared by all sequences, and per sequence the pages
+ * that hold it. Token t of sequence b is row t % page_size of page
+ * block_table[b, t / page_size] (device int32 [n_seqs, max_pages], entries
+ * past a sequence's pages are not read). seq_lens (device int32 [n_seqs]) is each
+ * sequence's length with the step's new tokens included. The new tokens' rows
+ * are token-major, [n_tokens, heads, head_dim]: with cu_q (device int32
+ * [n_seqs + 1], ascending from 0) sequence b has rows cu_q[b] .. cu_q[b + 1]
+ * - 1, at positions seq_lens[b] - (cu_q[b + 1] - row); without it (NULL, n_tokens
+ * == n_seqs) row b is sequence b's one new token, at position seq_lens[b] - 1.
+ * Rows past cu_q[n_seqs], and, without cu_q, the rows of sequences of length 0 (a
+ * padded batch) are no tokens.
+ * All of it is read on the device, so a captured call serves any batch of its
+ * sizes, and checked there: where a position has no entry in the table, an entry
+ * is outside [0, n_pages), or a sequence is shorter than its new tokens, 1 is
+ * stored to `bad_page_flag` (device int32, optional), nothing is written to or read
+ * from the cache for such a position, and a key there takes no part.
+ * The layout is the contiguous cache's with pages as its outer axis: a [n_kv,
+ * max_seq, head_dim] cache is a pool of one page of max_seq tokens.
+ * page_size >= 1 and any n_pages with n_pages · n_kv_heads · page_size < 2^32 - 1. */
+
+/* sph_rope_kv_append_tokens into a paged cache: q (rotated, into q_out, which is
+ * token-major here and may be q itself), k (rotated) and v of every new token,
+ * after the optional biases, the token's angle being its position's. Values
+ * equal sph_rope_kv_append_tokens's at the same positions bit for bit; types,
+ * biases, alignment and layout rules are its own. Replaces, per sequence of a
+ * batch, the chunk sequence of WgpuForwardEngine::forward_chunk
+ * (crates/sapient-models/src/forward/wgpu_engine.rs:525-573), whose cache is one
+ * contiguous block (crates/sapient-backends/wgpu/src/resident.rs:645-711). Rows
+ * of q_out that are no tokens, or that belong to a sequence shorter than its new
+ * tokens and have no position, are left as they were. */
+int sph_rope_kv_append_paged(const void* q, void* q_out, int64_t n_q_heads, const void* k, const void* v,
+                             int64_t n_kv_heads, int dtype, int layout, const int32_t* cu_q, const int32_t* seq_lens,
+                             const int32_t* block_table, int64_t n_seqs, int64_t max_pages, int64_t n_tokens,
+                             int64_t head_dim, float base, float pos_scale, void* kcache, void* vcache, int cache_dtype,
+                             int64_t n_pages, int64_t page_size, const void* bq, const void* bk, const void* bv,
+                             int bias_dtype, int32_t* bad_page_flag, void* stream);
+
+/* Softmax attention of one new token per sequence over a paged cache: q and
+ * out [n_seqs, n_q_heads, head_dim], query head h reading kv head h /
+ * (n_q_heads / n_kv_heads). Per key at position p <= the query's position P:
+ *   s = scale · q·k;  softcap > 0: s = softcap · tanh(s / softcap);
+ *   slopes (device f32 [n_q_heads], optional): s = s - slopes[h] · |P - p|;
+ * window > 0: only keys with P - p < window take part (0: all). out = sum of
+ * softmax(s) · v; a row without keys is zeros. Replaces the decode form of
+ * WgpuContext::attention (crates/sapient-backends/wgpu/src/resident.rs, shader
+ * attention.wgsl, grouped query heads), which the decode engine takes as a callback.
+ * dtype ∈ {F32, F16, BF16} for q and out; cache_dtype ∈ {F32, F16, BF16};
+ * head_dim a multiple of 8, at most 256; q, out, kcache and vcache 16-byte
+ * aligned; n_q_heads a multiple of n_kv_heads; scale finite. Sums and
+ * softmax statistics are f32. workspace: device memory of
+ * sph_paged_attention_workspace bytes, 16-byte aligned, whose contents need not be
+ * kept between calls, of one stream at a time. `out` may be q. */
+int sph_paged_attention(const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype,
+                        const int32_t* seq_lens, const int32_t* block_table, int64_t n_seqs, int64_t max_pages,
+                        int64_t head_dim, const void* kcache, const void* vcache, int cache_dtype, int64_t n_pages,
+                        int64_t page_size, float scale, float softcap, int64_t window, const float* slopes,
+                        void* workspace, int64_t workspace_bytes, int32_t* bad_page_flag, void* stream);
+
+/* The same for n_tokens rows of ragged chunks (cu_q as above, required): q and
+ * out [n_tokens, n_q_heads, head_dim]; the row at position P of sequence b reads
+ * the keys p of its own sequence with p <= P or p < prefix_lens[b] (device int32
+ * [n_seqs], optional: a prefix whose tokens see one another), P - p < window and p <
+ * seq_lens[b]. The chunk's own keys are in the cache already
+ * (sph_rope_kv_append_paged). Rows past cu_q[n_seqs] are left as they were.
+ * Replaces the chunk form of WgpuContext::attention (as above; causal,
+ * crates/sapient-models/src/forward/wgpu_engine.rs:575-607). workspace:
+ * sph_paged_attention_chunk_workspace bytes. `out` must not overlap q. */
+int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype,
+                              const int32_t* cu_q, const int32_t* seq_lens, const int32_t* block_table, int64_t n_seqs,
+                              int64_t max_pages, int64_t n_tokens, int64_t head_dim, const void* kcache,
+                              const void* vcache, int cache_dtype, int64_t n_pages, int64_t page_size, float scale,
+                              float softcap, int64_t window, const float* slopes, const int32_t* prefix_lens,
+                              void* workspace, int64_t workspace_bytes, int32_t* bad_page_flag, void* stream);
+
+/* Host functions: the workspace of the two calls at these sizes, in bytes (0 or
+ * more; negative: a status, for sizes the calls refuse). */
+int64_t sph_paged_attention_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_pages,
+                                      int64_t page_size, int64_t head_dim);
+int64_t sph_paged_attention_chunk_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_pages,
+                                            int64_t page_size, int64_t n_tokens, int64_t head_dim);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,6 +70,14 @@ SIGNATURES = {
     "sph_kv_append": (_i32, [_vp, _i32, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp]),
     "sph_kv_cache_update": (_i32, [_vp, _i32, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
     "sph_kv_cache_update_into": (_i32, [_vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "sph_rope_kv_append_paged": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i64,
+                                        _i64, _f, _f, _vp, _vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _vp, _vp]),
+    "sph_paged_attention": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _i64, _f,
+                                   _f, _i64, _vp, _vp, _i64, _vp, _vp]),
+    "sph_paged_attention_chunk": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp,
+                                         _i32, _i64, _i64, _f, _f, _i64, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "sph_paged_attention_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "sph_paged_attention_chunk_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     # sapient_hip_engine.h
     "sph_engine_create": (_i32, [C.POINTER(EngineConfig), _vp, _i32, _i64, C.POINTER(EngineLayer), _vp, PROJECT_FN,
                                  ATTEND_FN, _vp, C.POINTER(_vp)]),

@@ -14,12 +14,14 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <string>
 
 #include "sapient_hip.h"
@@ -539,6 +541,152 @@ PyObject* rope_kv_append_tokens(PyObject* const* a) {
     return out.object();
 }
 
+// A paged cache and its tables: pools [pages, n_kv, page_size, D], seq_lens [B], block_table [B, max_pages].
+struct Paged {
+    c10::DeviceGuard guard;  // the launches go to q's device, whichever is current
+    const Tensor *kc, *vc, *lens, *table;
+    const Tensor* cu = nullptr;
+    int64_t n_seqs, max_pages, n_pages, page_size;
+    int32_t* fl;
+    int cd;
+    Paged(const Tensor& q, PyObject* kco, PyObject* vco, PyObject* lo, PyObject* to, PyObject* cuo, PyObject* f, int64_t Hkv)
+        : guard(q.device()), kc(&dev(kco, "kcache")), vc(&dev(vco, "vcache")), lens(&dev(lo, "seq_lens")), table(&dev(to, "block_table")) {
+        if (kc->dim() != 4 || kc->sizes() != vc->sizes() || kc->size(3) != q.size(2) || kc->scalar_type() != vc->scalar_type() ||
+            (Hkv >= 0 && kc->size(1) != Hkv))
+            bad("caches must be [pages, Hkv, page_size, D] of one dtype");
+        if (lens->scalar_type() != ScalarType::Int || lens->dim() != 1) bad("seq_lens must be int32 [B]");
+        n_seqs = lens->size(0);
+        if (table->scalar_type() != ScalarType::Int || table->dim() != 2 || table->size(0) != n_seqs)
+            bad("block_table must be int32 [B, max_pages]");
+        max_pages = table->size(1);
+        n_pages = kc->size(0);
+        page_size = kc->size(2);
+        if (cuo != Py_None) {
+            cu = &dev(cuo, "cu_q");
+            if (cu->scalar_type() != ScalarType::Int || cu->numel() != n_seqs + 1) bad("cu_q must be int32 [B + 1]");
+        } else if (q.size(0) != n_seqs) {
+            bad("without cu_q there is one row per sequence");
+        }
+        fl = flag(f, "bad_page_flag");
+        cd = code(kc->scalar_type());
+        for (const Tensor* t : {kc, vc, lens, table, cu}) same_device(t, q);
+    }
+    static void same_device(const Tensor* t, const Tensor& q) {
+        if (t && t->device() != q.device()) bad("all tensors of a call must be on one device");
+    }
+};
+const int32_t* i32(const Tensor* t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; }
+
+// (q, k, v, seq_lens, block_table, base, kcache, vcache, cu_q, pos_scale, interleaved, bad_page_flag, bq, bk, bv, out)
+PyObject* rope_kv_append_paged(PyObject* const* a) {
+    const Tensor &q = dev(a[0], "q"), &k = dev(a[1], "k"), &v = dev(a[2], "v");
+    if (q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || q.size(0) != k.size(0) || q.size(2) != k.size(2))
+        bad("q must be [T, Hq, D] and k, v [T, Hkv, D]");
+    if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) bad("q, k and v must share dtype");
+    const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
+    const Paged p(q, a[6], a[7], a[3], a[4], a[8], a[11], Hkv);
+    const Tensor* b[3] = {vec(a[12], Hq * D, "bq"), vec(a[13], Hkv * D, "bk"), vec(a[14], Hkv * D, "bv")};
+    const Tensor* first = nullptr;
+    for (const Tensor* t : b) {
+        if (!t) continue;
+        if (first && t->scalar_type() != first->scalar_type()) bad("biases must share dtype");
+        first = t;
+    }
+    const int bd = first ? code(first->scalar_type()) : 0;
+    Out out(a[15], {T, Hq, D}, q.scalar_type(), q.device());
+    for (const Tensor* t : {&k, &v, b[0], b[1], b[2], (const Tensor*)&out.t}) p.same_device(t, q);
+    const int layout = truth(a[10]) ? SPH_ROPE_INTERLEAVED : SPH_ROPE_NEOX, d = code(q.scalar_type());
+    const float base = real(a[5]), scale = real(a[9]);
+    void *qp = ptr(q), *op = ptr(out.t), *kp = ptr(k), *vp = ptr(v), *kc = ptr(p.kc), *vc = ptr(p.vc), *bq = ptr(b[0]),
+         *bk = ptr(b[1]), *bv = ptr(b[2]), *st = stream_of(q);
+    const int32_t *cu = i32(p.cu), *lens = i32(p.lens), *table = i32(p.table);
+    call("rope_kv_append_paged", [&] {
+        return sph_rope_kv_append_paged(qp, op, Hq, kp, vp, Hkv, d, layout, cu, lens, table, p.n_seqs, p.max_pages, T, D,
+                                        base, scale, kc, vc, p.cd, p.n_pages, p.page_size, bq, bk, bv, bd, p.fl, st);
+    });
+    return out.object();
+}
+
+// What both attention calls take beside the tables.
+struct Attention {
+    const Tensor& q;
+    int64_t T, Hq, D;
+    float scale, cap;
+    int64_t window;
+    const Tensor* slopes;
+    Attention(PyObject* qo, PyObject* so, PyObject* co, PyObject* wo, PyObject* slo) : q(dev(qo, "q")) {
+        if (q.dim() != 3) bad("q must be [T, Hq, D]");
+        T = q.size(0);
+        Hq = q.size(1);
+        D = q.size(2);
+        scale = so == Py_None ? (float)(1.0 / std::sqrt((double)D)) : real(so);
+        cap = real(co);
+        window = as_integer(wo);
+        slopes = slo == Py_None ? nullptr : &dev(slo, "slopes");
+        if (slopes && (slopes->scalar_type() != ScalarType::Float || slopes->numel() != Hq)) bad("slopes must be f32 [Hq]");
+    }
+};
+
+// The caller's workspace, or one of `bytes` for the call.
+Tensor workspace(PyObject* o, int64_t bytes, at::Device device) {
+    if (o != Py_None) {
+        const Tensor& t = dev(o, "workspace");
+        if (t.scalar_type() != ScalarType::Byte || t.device() != device) bad("workspace must be uint8 on q's device");
+        return t;
+    }
+    if (bytes <= 0) return Tensor();
+    const NoGil release;
+    return at::empty({bytes}, at::TensorOptions().dtype(ScalarType::Byte).device(device));
+}
+
+// (q, kcache, vcache, seq_lens, block_table, scale, softcap, window, slopes, out, workspace, bad_page_flag)
+PyObject* paged_attention(PyObject* const* a) {
+    const Attention t(a[0], a[5], a[6], a[7], a[8]);
+    const Paged p(t.q, a[1], a[2], a[3], a[4], Py_None, a[11], -1);
+    Out out(a[9], {t.T, t.Hq, t.D}, t.q.scalar_type(), t.q.device());
+    for (const Tensor* x : {t.slopes, (const Tensor*)&out.t}) p.same_device(x, t.q);
+    const int64_t Hkv = p.kc->size(1);
+    const Tensor ws = workspace(
+        a[10], a[10] == Py_None ? sph_paged_attention_workspace(t.Hq, Hkv, p.n_seqs, p.max_pages, p.page_size, t.D) : 0,
+        t.q.device());
+    const int d = code(t.q.scalar_type());
+    void *qp = ptr(t.q), *op = ptr(out.t), *kc = ptr(p.kc), *vc = ptr(p.vc), *sl = ptr(t.slopes),
+         *wp = ws.defined() ? ptr(ws) : nullptr, *st = stream_of(t.q);
+    const int64_t wn = ws.defined() ? ws.numel() : 0;
+    const int32_t *lens = i32(p.lens), *table = i32(p.table);
+    call("paged_attention", [&] {
+        return sph_paged_attention(qp, op, t.Hq, Hkv, d, lens, table, p.n_seqs, p.max_pages, t.D, kc, vc, p.cd, p.n_pages,
+                                   p.page_size, t.scale, t.cap, t.window, static_cast<const float*>(sl), wp, wn, p.fl, st);
+    });
+    return out.object();
+}
+
+// (q, kcache, vcache, seq_lens, block_table, cu_q, scale, softcap, window, slopes, prefix_lens, out, workspace, bad_page_flag)
+PyObject* paged_attention_chunk(PyObject* const* a) {
+    const Attention t(a[0], a[6], a[7], a[8], a[9]);
+    if (a[5] == Py_None) raise(PyExc_TypeError, "cu_q must be a torch.Tensor");
+    const Paged p(t.q, a[1], a[2], a[3], a[4], a[5], a[13], -1);
+    const Tensor* prefix = a[10] == Py_None ? nullptr : &dev(a[10], "prefix_lens");
+    if (prefix && (prefix->scalar_type() != ScalarType::Int || prefix->numel() != p.n_seqs)) bad("prefix_lens must be int32 [B]");
+    Out out(a[11], {t.T, t.Hq, t.D}, t.q.scalar_type(), t.q.device());
+    for (const Tensor* x : {t.slopes, prefix, (const Tensor*)&out.t}) p.same_device(x, t.q);
+    const int64_t Hkv = p.kc->size(1);
+    const Tensor ws = workspace(
+        a[12], a[12] == Py_None ? sph_paged_attention_chunk_workspace(t.Hq, Hkv, p.n_seqs, p.max_pages, p.page_size, t.T, t.D) : 0,
+        t.q.device());
+    const int d = code(t.q.scalar_type());
+    void *qp = ptr(t.q), *op = ptr(out.t), *kc = ptr(p.kc), *vc = ptr(p.vc), *sl = ptr(t.slopes),
+         *wp = ws.defined() ? ptr(ws) : nullptr, *st = stream_of(t.q);
+    const int64_t wn = ws.defined() ? ws.numel() : 0;
+    const int32_t *cu = i32(p.cu), *lens = i32(p.lens), *table = i32(p.table), *pre = i32(prefix);
+    call("paged_attention_chunk", [&] {
+        return sph_paged_attention_chunk(qp, op, t.Hq, Hkv, d, cu, lens, table, p.n_seqs, p.max_pages, t.T, t.D, kc, vc,
+                                         p.cd, p.n_pages, p.page_size, t.scale, t.cap, t.window,
+                                         static_cast<const float*>(sl), pre, wp, wn, p.fl, st);
+    });
+    return out.object();
+}
+
 // ───────────────────────────── module ─────────────────────────────
 // No C++ exception leaves a function: torch's become Python errors.
 template <PyObject* (*F)(PyObject* const*), int N>
@@ -582,6 +730,9 @@ PyMethodDef kMethods[] = {SPH_OP(rms_norm, 5),
                           SPH_OP(kv_cache_update_into, 4),
                           SPH_OP(rope_kv_append, 13),
                           SPH_OP(rope_kv_append_tokens, 14),
+                          SPH_OP(rope_kv_append_paged, 16),
+                          SPH_OP(paged_attention, 12),
+                          SPH_OP(paged_attention_chunk, 14),
                           {"set_check", set_check, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 

@@ -1,0 +1,553 @@
+// attention.h — softmax attention over the paged KV cache: arguments, and the kernel of 16-column tiles that serves
+// single tokens, and chunks in every type (attention_decode.hip, attention_chunk.hip).
+//
+// Mathematics. For the rows (columns of a tile) that share a kv head, with s the capped and biased score in units
+// of log2 (scores times log2 e, so that a weight is one v_exp_f32):
+//   m = max s;  p = 2^(s - m);  l = sum p;  out = (sum p v) / l
+// in one pass over the keys: m is a running reference, raised (and l and the sums scaled by 2^(m_old - m_new))
+// only when a score passes it by 2^8, which keeps every p below 2^8 and spares most tiles the exchange between
+// lanes that a maximum needs. Parts of a key range (waves, workgroups) are joined by their (m, l, sums).
+//
+// Layout. Scores are computed transposed, S^T = K Q^T, so that lane (j = lane % 16, g = lane / 16) of a 16 x 16
+// matrix instruction holds column j's scores of tokens 4g .. 4g + 3, and keeps them as the second product's
+// operand O^T = V^T P^T without any exchange: the order of a product's inner dimension is free as long as both
+// operands share it, so V's rows are taken in the order in which the lanes hold P. A column's m and l live in
+// its own lanes. K and V go from memory to the operand registers with no stop in LDS: K as rows (lane j: token
+// j, 8 channels), V as rows too (lane j: channels E j .. E j + E - 1 of its tokens, E = DP / 16) and turned in
+// registers, one v_perm_b32 per two values, which leaves each lane with adjacent output channels.
+#pragma once
+
+#include "paged.h"
+#include "sph_common.h"
+
+namespace sph {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct AttnArgs {
+    const void* q;
+    void* out;
+    const void* kc;
+    const void* vc;
+    PagedTable pages;
+    const float* slopes;
+    const int32_t* prefix;
+    int32_t* bad;
+    int dtype;  // of q and out
+    int n_rows, nq, group, head_dim;
+    int window;  // 0: all keys
+    float scale, cap;
+};
+
+namespace {
+
+constexpr int kWave = 64;
+constexpr int kAttnWaves = 4;
+constexpr int kAttnThreads = kWave * kAttnWaves;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.0f;  // how far (log2) a score may pass the running reference
+constexpr float kNegInf = -__builtin_inff();
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// tanh of a score: by its own exp where the output is half precision (absolute error about 2^-23, under a rounding of
+// the weights), the library's where it is f32.
+template <bool ACCURATE>
+__device__ __forceinline__ float score_tanh(float x) {
+    if constexpr (ACCURATE) return tanhf(x);
+    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(exp2_hw(x * (2.0f * kLog2e)) + 1.0f);
+}
+
+template <typename TC>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (__is_same(TC, f16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+template <typename TC>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+    if constexpr (__is_same(TC, f16)) return narrow2_f16(a, b);
+    else return narrow2_bf16(a, b);
+}
+template <typename TC>
+__device__ __forceinline__ float widen_half(uint32_t w, int i) {
+    return widen(TC{(uint16_t)(w >> (16 * i))});
+}
+
+// Element i of a float tensor of type dt.
+__device__ __forceinline__ float load_as_f32(const void* p, int dt, size_t i) {
+    if (dt == SPH_F32) return static_cast<const float*>(p)[i];
+    const uint16_t h = static_cast<const uint16_t*>(p)[i];
+    return dt == SPH_F16 ? widen(f16{h}) : widen(bf16{h});
+}
+__device__ __forceinline__ void store4_from_f32(void* p, int dt, size_t i, f32x4 v) {
+    if (dt == SPH_F32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = v;
+    } else {
+        const u32x2 w = dt == SPH_F16 ? u32x2{narrow2_f16(v[0], v[1]), narrow2_f16(v[2], v[3])}
+                                      : u32x2{narrow2_bf16(v[0], v[1]), narrow2_bf16(v[2], v[3])};
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p) + i) = w;
+    }
+}
+
+// Which sequence the unit u falls to, where sequence b has count(b) units, counted by the block's NT threads: true,
+// with the sequence and the unit's number within it, or false past the last. Every thread calls it.
+struct Located {
+    int64_t wave_sum[kAttnThreads / kWave];
+    int64_t within;
+    int seq;
+};
+template <int NT, typename F>
+__device__ __forceinline__ bool locate_unit(int n_seqs, int64_t u, F count, Located& sm, int& seq, int64_t& within,
+                                            int64_t& total) {
+    const int tid = threadIdx.x, lane = tid % kWave;
+    const int each = (n_seqs + NT - 1) / NT, b0 = tid * each, b1 = b0 + each < n_seqs ? b0 + each : n_seqs;
+    int64_t own = 0;
+    for (int b = b0; b < b1; ++b) own += count(b);
+    int64_t upto = own;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const int64_t o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane == kWave - 1) sm.wave_sum[tid / kWave] = upto;
+    __syncthreads();
+    int64_t before = upto - own;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NT / kWave; ++w) {
+        if (w < tid / kWave) before += sm.wave_sum[w];
+        total += sm.wave_sum[w];
+    }
+    if (u >= before && u < before + own) {
+        int b = b0;
+        for (int64_t n; u >= before + (n = count(b)); ++b) before += n;
+        sm.seq = b;
+        sm.within = u - before;
+    }
+    __syncthreads();
+    if (u >= total) return false;
+    seq = sm.seq;
+    within = sm.within;
+    return true;
+}
+
+// A tile's 16 columns: the rows (token i of the sequence's new ones, head h · group + c) with number i · group + c in
+// [first, first + 16) of `rows`, for kv head h.
+struct Tile {
+    int seq, h, first, rows, row0;  // row0: the sequence's first row
+    int pos0;                       // position of the sequence's first new token
+};
+
+// HIGH: q is f32, or the cache's type is another one than q's. LOW: both the same half type.
+template <typename TC, int DP, bool EXACT, bool HIGH>
+struct TileKernel {
+    static constexpr int kDP = DP;
+    static constexpr bool kF32 = sizeof(TC) == 4;
+    static constexpr int ST = kF32 ? 16 : 32;              // tokens of a wave's step
+    static constexpr int E = DP / 16;                      // channels of V per lane
+    static constexpr int KB = ST / 16;                     // 16-token blocks
+    static constexpr int KS = kF32 ? DP / 16 : DP / 32;    // 16-byte pieces of a K row per lane
+    static constexpr int VT = ST / 4;                      // tokens of V per lane
+    static constexpr int VW = E * (int)sizeof(TC) / 4;     // words of V per token and lane
+    // Pieces of the cache's type that q and the weights are written as, high one first. q: exact (f16 and bf16 into
+    // one another; f32 into bf16), or within 2^-22 (f32 into f16). Weights: with one piece their rounding would add
+    // to the output's as much again, so two; three where the output is f32 and a piece has 8 bits.
+    static constexpr int NQ = kF32 ? 1 : !HIGH ? 1 : __is_same(TC, bf16) ? 3 : 2;
+    static constexpr int NP = kF32 ? 1 : HIGH && __is_same(TC, bf16) ? 3 : 2;
+    // An f16 weight below 2^-14 loses bits: the reference is taken 2^7 lower, so that weights run up to 2^15.
+    static constexpr float kLift = __is_same(TC, f16) ? 7.0f : 0.0f;
+    static constexpr int kPasses = DP > 128 ? DP / 128 : 1;  // of the join over waves, 128 channels each
+    static constexpr int kJoin = DP / kPasses, kJoinRow = kJoin + 4;
+
+    struct Shared {
+        float m[kAttnWaves][16], l[kAttnWaves][16];
+        float acc[kAttnWaves][16][kJoinRow];  // rows padded: 16-byte writes of 8 neighbouring columns hit all banks
+        Located located;
+    };
+
+    using KRegs = u32x4[KB][KS];
+    using VRegs = uint32_t[VT][VW];
+
+    // One column's state in its lanes.
+    float m, l;
+    f32x4 acc[E];
+
+    // The keys [lo, hi) of the tile, over the block's four waves; then store(column, channel, m, l, sums of 4 channels)
+    // for every column of the tile, by the block's threads.
+    template <typename Store>
+    __device__ __forceinline__ void attend(const AttnArgs& a, Shared& sm, const Tile& t, uint32_t lo, uint32_t hi, Store store) {
+        const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, j = lane % 16, g = lane / 16;
+        const int D = EXACT ? DP : a.head_dim;
+        const int n_cols = t.rows - t.first < 16 ? t.rows - t.first : 16;
+        const int col = t.first + (j < n_cols ? j : n_cols - 1), tok = col / a.group, head = t.h * a.group + (col - tok * a.group);
+        const int pos = t.pos0 + tok;
+        const int pos_first = t.pos0 + t.first / a.group, pos_last = t.pos0 + (t.first + n_cols - 1) / a.group;
+        const int prefix = a.prefix != nullptr ? a.prefix[t.seq] : 0;
+        const float slope = a.slopes != nullptr ? a.slopes[head] : 0.0f;
+
+        // q, as the B operand: column j, channels of this lane's k slots.
+        float unit = a.scale;
+        const size_t q_at = ((size_t)(t.row0 + tok) * (size_t)a.nq + (size_t)head) * (size_t)D;
+        u32x4 q[NQ][KS];
+        if constexpr (!HIGH && !kF32) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int d = 32 * s + 8 * g;
+                q[0][s] = u32x4{0, 0, 0, 0};
+                if (EXACT || d < D) q[0][s] = *reinterpret_cast<const u32x4*>(static_cast<const TC*>(a.q) + q_at + d);
+            }
+        } else if constexpr (kF32) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = 16 * s + 4 * g + e;
+                    q[0][s][e] = __float_as_uint(EXACT || d < D ? load_as_f32(a.q, a.dtype, q_at + d) : 0.0f);
+                }
+        } else {
+            // Brought to [1, 2) by a power of two, so that no piece leaves the type's range.
+            float f[KS][8], most = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int d = 32 * s + 8 * g + e;
+                    f[s][e] = EXACT || d < D ? load_as_f32(a.q, a.dtype, q_at + d) : 0.0f;
+                    most = fmaxf(most, fabsf(f[s][e]));
+                }
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const int ex = most > 0.0f && most < __builtin_inff() ? ilogbf(most) : 0;
+            unit = ldexpf(unit, ex);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    float x = ldexpf(f[s][e], -ex), y = ldexpf(f[s][e + 1], -ex);
+#pragma unroll
+                    for (int p = 0; p < NQ; ++p) {
+                        const uint32_t w = narrow2<TC>(x, y);
+                        q[p][s][e / 2] = w;
+                        x -= widen_half<TC>(w, 0);
+                        y -= widen_half<TC>(w, 1);
+                    }
+                }
+        }
+
+        const TC *kc = static_cast<const TC*>(a.kc), *vc = static_cast<const TC*>(a.vc);
+        const uint32_t head_rows = (uint32_t)t.h * a.pages.page.d;
+        // Pool row of the step's token that this lane follows, or kNoRow outside [lo, hi) and where there is no page.
+        auto row_at = [&](uint32_t t0) -> uint32_t {
+            const uint32_t k = t0 + (uint32_t)(lane % ST);
+            if (k < lo || k >= hi) return kNoRow;
+            const uint32_t r = a.pages.row(t.seq, k);
+            if (r == kNoRow) {
+                if (a.bad != nullptr) *a.bad = 1;
+                return kNoRow;
+            }
+            return r + head_rows;
+        };
+        // Row 0 stands in for a missing one: there to be read, and masked or cleared.
+        auto load_k = [&](uint32_t rows, KRegs& k) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                const uint32_t r = __shfl(rows, 16 * b + j);
+                const TC* p = kc + (size_t)(r == kNoRow ? 0u : r) * (size_t)D;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int d = kF32 ? 16 * s + 4 * g : 32 * s + 8 * g;
+                    k[b][s] = u32x4{0, 0, 0, 0};
+                    if (EXACT || d < D) k[b][s] = *reinterpret_cast<const u32x4*>(p + d);
+                }
+            }
+        };
+        auto load_v = [&](uint32_t rows, VRegs& v) {
+#pragma unroll
+            for (int e = 0; e < VT; ++e) {
+                const uint32_t r = __shfl(rows, 16 * (e / 4) + 4 * g + e % 4);
+                const TC* p = vc + (size_t)(r == kNoRow ? 0u : r) * (size_t)D + E * j;
+                constexpr int B = VW >= 4 ? 4 : 2;  // words per access
+#pragma unroll
+                for (int c = 0; c < VW / B; ++c) {
+                    const int d = c * (B * 4 / (int)sizeof(TC));
+                    if (EXACT || E * j + d < D) {
+                        if constexpr (B == 4) {
+                            const u32x4 w = *reinterpret_cast<const u32x4*>(p + d);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[e][4 * c + i] = w[i];
+                        } else {
+                            const u32x2 w = *reinterpret_cast<const u32x2*>(p + d);
+                            v[e][0] = w[0];
+                            v[e][1] = w[1];
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < B; ++i) v[e][B * c + i] = 0u;
+                    }
+                }
+            }
+        };
+
+        m = kNegInf;
+        l = 0.0f;
+#pragma unroll
+        for (int n = 0; n < E; ++n) acc[n] = f32x4{0, 0, 0, 0};
+
+        constexpr uint32_t kStep = ST * kAttnWaves;
+        KRegs k;
+        VRegs v;
+        uint32_t t0 = (lo & ~(uint32_t)(ST - 1)) + (uint32_t)(wave * ST);
+        uint32_t rows = row_at(t0), rows_next = row_at(t0 + kStep);
+        if (t0 < hi) load_k(rows, k);
+        for (; t0 < hi; t0 += kStep) {
+            const uint32_t rows_after = row_at(t0 + 2 * kStep);
+            load_v(rows, v);
+            KRegs k_next;
+            if (t0 + kStep < hi) load_k(rows_next, k_next);
+
+            f32x4 s[KB];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                s[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < KS; ++c) {
+                    if constexpr (kF32) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[b][c][e]),
+                                                                        __uint_as_float(q[0][c][e]), s[b], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int p = NQ - 1; p >= 0; --p) s[b] = mma<TC>(k[b][c], q[p][c], s[b]);
+                    }
+                }
+            }
+
+            // Scores in log2 units, and the mask where the step is not all visible to all columns.
+            const uint32_t there = (uint32_t)__ballot(rows != kNoRow) & (uint32_t)((uint64_t(1) << ST) - 1);
+            const bool whole = there == (uint32_t)((uint64_t(1) << ST) - 1);
+            const uint32_t last = t0 + ST - 1;
+            const bool seen = whole && pos_first >= 0 && ((int)last <= pos_first || (int)last < prefix) &&
+                              (a.window == 0 || pos_last - (int)t0 < a.window);
+            if (a.cap == 0.0f && a.slopes == nullptr) {
+                const float c = unit * kLog2e;
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[b][r] *= c;
+            } else {
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float x = s[b][r] * unit;
+                        if (a.cap != 0.0f) x = a.cap * score_tanh<HIGH || kF32>(x / a.cap);
+                        if (a.slopes != nullptr) x -= slope * fabsf((float)(pos - (int)(t0 + 16 * b + 4 * g + r)));
+                        s[b][r] = x * kLog2e;
+                    }
+            }
+            if (!seen) {
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 16 * b + 4 * g + r, p = (int)t0 + i;
+                        const bool see = ((there >> i) & 1) && pos >= 0 && (p <= pos || p < prefix) &&
+                                         (a.window == 0 || pos - p < a.window);
+                        if (!see) s[b][r] = kNegInf;
+                    }
+            }
+            if (!whole) {  // what lies in a row that is no key of the sequence may be anything, and 0 · inf is not 0
+#pragma unroll
+                for (int e = 0; e < VT; ++e)
+                    if (!((there >> (16 * (e / 4) + 4 * g + e % 4)) & 1)) {
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) v[e][w] = 0u;
+                    }
+            }
+
+            float top = s[0][0];
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[b][r]);
+            if (__any(top > m + (kLift + kSlack))) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float m_new = fmaxf(m, top - kLift);
+                const float f = m_new == kNegInf ? 1.0f : exp2_hw(m - m_new);
+                m = m_new;
+                l *= f;
+#pragma unroll
+                for (int n = 0; n < E; ++n) acc[n] *= f;
+            }
+            const float ref = m == kNegInf ? 0.0f : m;
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[b][r] = exp2_hw(s[b][r] - ref);
+                    l += s[b][r];
+                }
+
+            if constexpr (kF32) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int n = 0; n < E; ++n)
+                        acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][n]), s[0][r], acc[n], 0, 0, 0);
+            } else {
+                u32x4 p[NP];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // k slots 2i, 2i + 1 of this lane
+                    float x = s[i / 2][2 * (i % 2)], y = s[i / 2][2 * (i % 2) + 1];
+#pragma unroll
+                    for (int c = 0; c < NP; ++c) {
+                        const uint32_t w = narrow2<TC>(x, y);
+                        p[c][i] = w;
+                        x -= widen_half<TC>(w, 0);
+                        y -= widen_half<TC>(w, 1);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < E; ++n) {
+                    u32x4 w;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = __builtin_amdgcn_perm(v[2 * i + 1][n / 2], v[2 * i][n / 2], n % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                    for (int c = NP - 1; c >= 0; --c) acc[n] = mma<TC>(w, p[c], acc[n]);
+                }
+            }
+            rows = rows_next;
+            rows_next = rows_after;
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int c = 0; c < KS; ++c) k[b][c] = k_next[b][c];
+        }
+
+        // The four waves' parts. Lane (j, g) holds column j, channels E (4g + r) + n in acc[n][r].
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        __syncthreads();  // the block's last tile has been read
+        if (g == 0) {
+            sm.m[wave][j] = m;
+            sm.l[wave][j] = l;
+        }
+        constexpr int EP = E < 8 ? E : 8;  // channels of a lane's run in a pass
+#pragma unroll
+        for (int pass = 0; pass < kPasses; ++pass) {
+            if (pass > 0) __syncthreads();
+            if (j < n_cols) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int n = 0; n < EP; n += 4)
+                        *reinterpret_cast<f32x4*>(&sm.acc[wave][j][EP * (4 * g + r) + n]) =
+                            f32x4{acc[8 * pass + n][r], acc[8 * pass + n + 1][r], acc[8 * pass + n + 2][r], acc[8 * pass + n + 3][r]};
+            }
+            __syncthreads();
+            constexpr int kLanes = kJoin / 4;  // threads of a column
+            for (int c = tid / kLanes; c < n_cols; c += kAttnThreads / kLanes) {
+                const int x = 4 * (tid % kLanes);
+                const int d = kPasses == 1 ? x : 16 * (x / 8) + 8 * pass + x % 8;
+                float top = kNegInf;
+#pragma unroll
+                for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, sm.m[w][c]);
+                float total = 0.0f;
+                f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < kAttnWaves; ++w) {
+                    const float f = sm.m[w][c] == kNegInf ? 0.0f : exp2_hw(sm.m[w][c] - top);
+                    const f32x4 part = *reinterpret_cast<const f32x4*>(&sm.acc[w][c][x]);
+                    total = __builtin_fmaf(sm.l[w][c], f, total);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(part[i], f, sum[i]);
+                }
+                if (EXACT || d < D) store(c, d, top, total, sum);
+            }
+        }
+    }
+};
+
+// The keys that any column of the tile may see, [lo, hi).
+__device__ __forceinline__ void key_range(const AttnArgs& a, const Tile& t, int len, uint32_t& lo, uint32_t& hi) {
+    const int last_col = t.first + 15 < t.rows ? t.first + 15 : t.rows - 1;
+    const int pos_first = t.pos0 + t.first / a.group, pos_last = t.pos0 + last_col / a.group;
+    const int prefix = a.prefix != nullptr ? a.prefix[t.seq] : 0;
+    int end = pos_last + 1 > prefix ? pos_last + 1 : prefix;
+    if (pos_last < 0) end = 0;
+    if (end > len) end = len;
+    int begin = a.window > 0 && pos_first - a.window + 1 > 0 ? pos_first - a.window + 1 : 0;
+    hi = end < 0 ? 0u : (uint32_t)end;
+    lo = (uint32_t)begin < hi ? (uint32_t)begin : hi;
+}
+
+template <typename K>
+__global__ __launch_bounds__(kAttnThreads, K::kDP > 128 ? 1 : 2) void paged_tiles_kernel(AttnArgs a, int tiles_per_seq) {
+    __shared__ typename K::Shared sm;
+    const int n_kv = a.pages.n_kv;
+    Tile t;
+    t.h = blockIdx.x % n_kv;
+    int64_t unit = blockIdx.x / n_kv;
+    int begin, end;
+    if (a.pages.cu == nullptr) {
+        t.seq = (int)(unit / tiles_per_seq);
+        unit -= (int64_t)t.seq * tiles_per_seq;
+        begin = t.seq;
+        end = begin + 1;
+    } else {
+        auto tiles = [&](int b) -> int64_t {
+            int lo, hi;
+            a.pages.new_rows(b, a.n_rows, lo, hi);
+            return ((int64_t)(hi - lo) * a.group + 15) / 16;
+        };
+        int64_t total;
+        if (!locate_unit<kAttnThreads>(a.pages.n_seqs, unit, tiles, sm.located, t.seq, unit, total)) return;
+        a.pages.new_rows(t.seq, a.n_rows, begin, end);
+    }
+    const int len = a.pages.lens[t.seq];
+    t.row0 = begin;
+    t.rows = (end - begin) * a.group;
+    t.first = 16 * (int)unit;
+    t.pos0 = len - (end - begin);
+    if (a.bad != nullptr && a.pages.cu != nullptr && t.pos0 < 0 && threadIdx.x == 0) *a.bad = 1;
+    uint32_t lo, hi;
+    key_range(a, t, len, lo, hi);
+    K k;
+    k.attend(a, sm, t, lo, hi, [&](int c, int d, float, float total, f32x4 sum) {
+        const int col = t.first + c, tok = col / a.group, head = t.h * a.group + (col - tok * a.group);
+        const float f = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = total == 0.0f ? 0.0f : sum[i] * f;
+        store4_from_f32(a.out, a.dtype, ((size_t)(t.row0 + tok) * (size_t)a.nq + (size_t)head) * (size_t)a.head_dim + d, sum);
+    });
+}
+
+// The kernel of a cache type, the narrowest that holds head_dim.
+template <typename TC, bool HIGH, typename F>
+int with_tile_kernel(int head_dim, F&& f) {
+    if (head_dim == 64) return f(TileKernel<TC, 64, true, HIGH>{});
+    if (head_dim == 128) return f(TileKernel<TC, 128, true, HIGH>{});
+    if (head_dim == 256) return f(TileKernel<TC, 256, true, HIGH>{});
+    if (head_dim < 64) return f(TileKernel<TC, 64, false, HIGH>{});
+    if (head_dim < 128) return f(TileKernel<TC, 128, false, HIGH>{});
+    return f(TileKernel<TC, 256, false, HIGH>{});
+}
+
+}  // namespace
+
+// The checks of both entry points; fills `a`.
+int attn_args(AttnArgs& a, const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype, const int32_t* cu_q,
+              const int32_t* seq_lens, const int32_t* block_table, int64_t n_seqs, int64_t max_pages, int64_t n_rows,
+              int64_t head_dim, const void* kcache, const void* vcache, int cache_dtype, int64_t n_pages,
+              int64_t page_size, float scale, float softcap, int64_t window, const float* slopes,
+              const int32_t* prefix_lens, int32_t* bad) __attribute__((visibility("hidden")));
+
+}  // namespace sph

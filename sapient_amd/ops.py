@@ -198,6 +198,61 @@ def kv_cache_update_into(src: torch.Tensor, cache: torch.Tensor, out: torch.Tens
     return _native.kv_cache_update_into(src, cache, out, cur_len)
 
 
+def rope_kv_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_lens: torch.Tensor,
+                         block_table: torch.Tensor, base: float, kcache: torch.Tensor, vcache: torch.Tensor,
+                         cu_q: Optional[torch.Tensor] = None, pos_scale: float = 1.0, interleaved: bool = False,
+                         bad_page_flag: Optional[torch.Tensor] = None, bq: Optional[torch.Tensor] = None,
+                         bk: Optional[torch.Tensor] = None, bv: Optional[torch.Tensor] = None,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The fused step of a batch into a paged cache: q [T, Hq, D], k/v [T, Hkv, D] (the new tokens' rows);
+    caches [pages, Hkv, page_size, D]; seq_lens int32 [B], the new tokens included; block_table int32
+    [B, max_pages]; cu_q int32 [B + 1], the rows of each sequence (None: one row per sequence, T == B). Returns
+    the rotated q [T, Hq, D] (`out` may be q); rows that are no tokens are left as they were (in a fresh
+    output: undefined). bad_page_flag (int32) receives 1 where a position has no page in the pool, or a sequence is
+    shorter than its new tokens (wgpu_engine.rs:525-573 per sequence)."""
+    return _native.rope_kv_append_paged(q, k, v, seq_lens, block_table, base, kcache, vcache, cu_q, pos_scale,
+                                        interleaved, bad_page_flag, bq, bk, bv, out)
+
+
+def paged_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, seq_lens: torch.Tensor,
+                    block_table: torch.Tensor, scale: Optional[float] = None, softcap: float = 0.0, window: int = 0,
+                    slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None,
+                    bad_page_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence, q [B, Hq, D], over the pages (as rope_kv_append_paged; the
+    tokens' own keys are there already): softmax of scale * q.k (default D ** -0.5), capped by softcap * tanh(s /
+    softcap), less slopes[h] (f32 [Hq]) times the distance, over the last `window` keys (0: all). Rows of
+    sequences of length 0 are zeros. workspace: paged_attention_workspace bytes of uint8 to reuse on one stream
+    (None: allocated for the call). `out` may be q."""
+    return _native.paged_attention(q, kcache, vcache, seq_lens, block_table, scale, softcap, window, slopes, out,
+                                   workspace, bad_page_flag)
+
+
+def paged_attention_chunk(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, seq_lens: torch.Tensor,
+                          block_table: torch.Tensor, cu_q: torch.Tensor, scale: Optional[float] = None,
+                          softcap: float = 0.0, window: int = 0, slopes: Optional[torch.Tensor] = None,
+                          prefix_lens: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                          workspace: Optional[torch.Tensor] = None,
+                          bad_page_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_attention for ragged chunks: q [T, Hq, D], rows cu_q[b] .. cu_q[b + 1] being sequence b's new tokens.
+    A row sees its sequence's keys up to its own position, and all below prefix_lens[b] (int32 [B]). Rows past
+    cu_q[B] are left as they were (in a fresh output: undefined)."""
+    return _native.paged_attention_chunk(q, kcache, vcache, seq_lens, block_table, cu_q, scale, softcap, window, slopes,
+                                         prefix_lens, out, workspace, bad_page_flag)
+
+
+def paged_attention_workspace(n_q_heads: int, n_kv_heads: int, n_seqs: int, max_pages: int, page_size: int, head_dim: int,
+                              n_tokens: Optional[int] = None) -> int:
+    """Bytes of workspace of paged_attention at these sizes, or, given n_tokens, of paged_attention_chunk."""
+    if n_tokens is None:
+        n = lib().sph_paged_attention_workspace(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim)
+    else:
+        n = lib().sph_paged_attention_chunk_workspace(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, n_tokens,
+                                                      head_dim)
+    check(min(n, 0), "paged_attention_workspace")
+    return n
+
+
 def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, base: float,
                    kcache: torch.Tensor, vcache: torch.Tensor, pos_scale: float = 1.0, interleaved: bool = False,
                    bad_pos_flag: Optional[torch.Tensor] = None, bq: Optional[torch.Tensor] = None,
