@@ -94,15 +94,15 @@ __device__ __forceinline__ void store4_from_f32(void* p, int dt, size_t i, f32x4
     }
 }
 
-// Which sequence the unit u falls to, where sequence b has count(b) units, counted by the block's NT threads: true,
-// with the sequence and the unit's number within it, or false past the last. Every thread calls it.
+// Which sequence the unit pick(total) falls to, where sequence b has count(b) units, counted by the block's NT threads:
+// true, with the sequence and the unit's number within it, or false past the last. Every thread calls it.
 struct Located {
     int64_t wave_sum[kAttnThreads / kWave];
     int64_t within;
     int seq;
 };
-template <int NT, typename F>
-__device__ __forceinline__ bool locate_unit(int n_seqs, int64_t u, F count, Located& sm, int& seq, int64_t& within,
+template <int NT, typename F, typename P>
+__device__ __forceinline__ bool locate_unit(int n_seqs, P pick, F count, Located& sm, int& seq, int64_t& within,
                                             int64_t& total) {
     const int tid = threadIdx.x, lane = tid % kWave;
     const int each = (n_seqs + NT - 1) / NT, b0 = tid * each, b1 = b0 + each < n_seqs ? b0 + each : n_seqs;
@@ -123,6 +123,7 @@ __device__ __forceinline__ bool locate_unit(int n_seqs, int64_t u, F count, Loca
         if (w < tid / kWave) before += sm.wave_sum[w];
         total += sm.wave_sum[w];
     }
+    const int64_t u = pick(total);
     if (u >= before && u < before + own) {
         int b = b0;
         for (int64_t n; u >= before + (n = count(b)); ++b) before += n;
@@ -149,6 +150,8 @@ struct TileKernel {
     static constexpr int kDP = DP;
     static constexpr bool kF32 = sizeof(TC) == 4;
     static constexpr int ST = kF32 ? 16 : 32;              // tokens of a wave's step
+    static constexpr int kStep = ST * kAttnWaves;          // and of the block's
+    static constexpr int kBlocksPerCu = DP > 128 ? 1 : 2;  // by registers
     static constexpr int E = DP / 16;                      // channels of V per lane
     static constexpr int KB = ST / 16;                     // 16-token blocks
     static constexpr int KS = kF32 ? DP / 16 : DP / 32;    // 16-byte pieces of a K row per lane
@@ -298,7 +301,6 @@ struct TileKernel {
 #pragma unroll
         for (int n = 0; n < E; ++n) acc[n] = f32x4{0, 0, 0, 0};
 
-        constexpr uint32_t kStep = ST * kAttnWaves;
         KRegs k;
         VRegs v;
         uint32_t t0 = (lo & ~(uint32_t)(ST - 1)) + (uint32_t)(wave * ST);
@@ -477,20 +479,20 @@ struct TileKernel {
 };
 
 // The keys that any column of the tile may see, [lo, hi).
-__device__ __forceinline__ void key_range(const AttnArgs& a, const Tile& t, int len, uint32_t& lo, uint32_t& hi) {
+__device__ __forceinline__ void key_range(const AttnArgs& a, const Tile& t, int keys, uint32_t& lo, uint32_t& hi) {
     const int last_col = t.first + 15 < t.rows ? t.first + 15 : t.rows - 1;
     const int pos_first = t.pos0 + t.first / a.group, pos_last = t.pos0 + last_col / a.group;
     const int prefix = a.prefix != nullptr ? a.prefix[t.seq] : 0;
     int end = pos_last + 1 > prefix ? pos_last + 1 : prefix;
     if (pos_last < 0) end = 0;
-    if (end > len) end = len;
+    if (end > keys) end = keys;
     int begin = a.window > 0 && pos_first - a.window + 1 > 0 ? pos_first - a.window + 1 : 0;
     hi = end < 0 ? 0u : (uint32_t)end;
     lo = (uint32_t)begin < hi ? (uint32_t)begin : hi;
 }
 
 template <typename K>
-__global__ __launch_bounds__(kAttnThreads, K::kDP > 128 ? 1 : 2) void paged_tiles_kernel(AttnArgs a, int tiles_per_seq) {
+__global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_tiles_kernel(AttnArgs a, int tiles_per_seq) {
     __shared__ typename K::Shared sm;
     const int n_kv = a.pages.n_kv;
     Tile t;
@@ -509,7 +511,7 @@ __global__ __launch_bounds__(kAttnThreads, K::kDP > 128 ? 1 : 2) void paged_tile
             return ((int64_t)(hi - lo) * a.group + 15) / 16;
         };
         int64_t total;
-        if (!locate_unit<kAttnThreads>(a.pages.n_seqs, unit, tiles, sm.located, t.seq, unit, total)) return;
+        if (!locate_unit<kAttnThreads>(a.pages.n_seqs, [&](int64_t) { return unit; }, tiles, sm.located, t.seq, unit, total)) return;
         a.pages.new_rows(t.seq, a.n_rows, begin, end);
     }
     const int len = a.pages.lens[t.seq];
@@ -519,7 +521,7 @@ __global__ __launch_bounds__(kAttnThreads, K::kDP > 128 ? 1 : 2) void paged_tile
     t.pos0 = len - (end - begin);
     if (a.bad != nullptr && a.pages.cu != nullptr && t.pos0 < 0 && threadIdx.x == 0) *a.bad = 1;
     uint32_t lo, hi;
-    key_range(a, t, len, lo, hi);
+    key_range(a, t, a.pages.keys(t.seq, a.bad, threadIdx.x == 0), lo, hi);
     K k;
     k.attend(a, sm, t, lo, hi, [&](int c, int d, float, float total, f32x4 sum) {
         const int col = t.first + c, tok = col / a.group, head = t.h * a.group + (col - tok * a.group);
@@ -528,6 +530,181 @@ __global__ __launch_bounds__(kAttnThreads, K::kDP > 128 ? 1 : 2) void paged_tile
         for (int i = 0; i < 4; ++i) sum[i] = total == 0.0f ? 0.0f : sum[i] * f;
         store4_from_f32(a.out, a.dtype, ((size_t)(t.row0 + tok) * (size_t)a.nq + (size_t)head) * (size_t)a.head_dim + d, sum);
     });
+}
+
+// ───────────────────────── single tokens, split ─────────────────────────
+// Few sequences of many keys, and batches of mixed lengths, leave CUs idle where a block takes a whole (sequence,
+// kv head): 131071 keys of 8 kv heads would run on 8 of 256 CUs. So the keys of all sequences are cut into units
+// of one block step, in the order sequence, tile of columns, step, and as many blocks as the GPU holds at once take
+// equal shares of them, each a run of neighbouring units: a few pieces of (sequence, tile) ranges, of which only the first
+// and the last can be part of one that other blocks share. Those go to the workspace, and paged_join_kernel sums
+// them in a fixed order. The shares follow the lengths on the device: nothing is read back, a captured call
+// serves any lengths.
+struct SplitArgs {
+    int tiles_per_seq;  // of 16 columns: (kv head, tile of its group)
+    int cols;           // of the widest tile
+    int shares;         // blocks
+    float* part;        // [2 · shares][cols][head_dim] sums, then [2 · shares][cols][2] m and l
+};
+
+// The key range of single token b, as steps from the aligned start.
+template <int STEP>
+struct SplitRange {
+    int len;
+    uint32_t lo, hi, start, steps;
+    __device__ __forceinline__ SplitRange(const AttnArgs& a, int b) {
+        len = a.pages.lens[b];
+        hi = (uint32_t)a.pages.keys(b, nullptr, false);
+        lo = a.window > 0 && len > a.window ? (uint32_t)(len - a.window) : 0u;
+        if (lo > hi) lo = hi;
+        start = lo & ~31u;
+        steps = (hi - start + STEP - 1) / STEP;
+        if (steps == 0) steps = 1;  // a row without keys is one unit: its zeros
+    }
+};
+
+// `shares` of `total` units, none of them empty.
+__device__ __forceinline__ int64_t share_count(int64_t total, int shares) { return total < shares ? total : shares; }
+__device__ __forceinline__ int64_t share_start(int64_t share, int64_t total, int64_t shares) { return share * total / shares; }
+// The share that unit u is in: the largest with share_start <= u.
+__device__ __forceinline__ int64_t share_of(int64_t u, int64_t total, int64_t shares) { return ((u + 1) * shares - 1) / total; }
+
+template <typename K>
+__global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_split_kernel(AttnArgs a, SplitArgs sp) {
+    __shared__ typename K::Shared sm;
+    const int share = blockIdx.x;
+    int seq;
+    int64_t within, total;
+    auto units = [&](int b) -> int64_t { return (int64_t)SplitRange<K::kStep>(a, b).steps * sp.tiles_per_seq; };
+    auto first = [&](int64_t n) { return share_start(share, n, share_count(n, sp.shares)); };
+    if (!locate_unit<kAttnThreads>(a.pages.n_seqs, first, units, sm.located, seq, within, total)) return;
+    const int64_t begin = first(total), end = share_start(share + 1, total, share_count(total, sp.shares));
+    const int tiles_per_head = sp.tiles_per_seq / a.pages.n_kv;
+    for (int64_t u = begin; u < end; ++seq, within = 0) {
+        const SplitRange<K::kStep> r(a, seq);
+        a.pages.keys(seq, a.bad, threadIdx.x == 0);
+        for (; u < end && within < (int64_t)r.steps * sp.tiles_per_seq;) {
+            const int tile = (int)(within / r.steps);
+            const uint32_t step = (uint32_t)(within - (int64_t)tile * r.steps);
+            uint32_t n = r.steps - step;
+            if ((int64_t)n > end - u) n = (uint32_t)(end - u);
+            Tile t;
+            t.seq = t.row0 = seq;
+            t.h = tile / tiles_per_head;
+            t.first = 16 * (tile - t.h * tiles_per_head);
+            t.rows = a.group;
+            t.pos0 = r.len - 1;
+            uint32_t lo = r.start + step * K::kStep, hi = lo + n * K::kStep;
+            if (lo < r.lo) lo = r.lo;
+            if (hi > r.hi) hi = r.hi;
+            K k;
+            if (n == r.steps) {
+                k.attend(a, sm, t, lo, hi, [&](int c, int d, float, float l, f32x4 sum) {
+                    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] = l == 0.0f ? 0.0f : sum[i] * f;
+                    const size_t row = (size_t)seq * (size_t)a.nq + (size_t)(t.h * a.group + t.first + c);
+                    store4_from_f32(a.out, a.dtype, row * (size_t)a.head_dim + d, sum);
+                });
+            } else {
+                const size_t slot = 2 * (size_t)share + (u == begin ? 0 : 1);
+                k.attend(a, sm, t, lo, hi, [&](int c, int d, float m, float l, f32x4 sum) {
+                    const size_t row = slot * (size_t)sp.cols + (size_t)c;
+                    *reinterpret_cast<f32x4*>(sp.part + row * (size_t)a.head_dim + d) = sum;
+                    if (d == 0) {
+                        float* ml = sp.part + 2 * (size_t)sp.shares * (size_t)sp.cols * (size_t)a.head_dim + 2 * row;
+                        ml[0] = m;
+                        ml[1] = l;
+                    }
+                });
+            }
+            u += n;
+            within += n;
+        }
+    }
+}
+
+// One block per (sequence, tile): nothing where one share held it, else the sum of its parts.
+template <int STEP>
+__global__ __launch_bounds__(kAttnThreads) void paged_join_kernel(AttnArgs a, SplitArgs sp) {
+    __shared__ Located located;
+    __shared__ f32x4 sums[kAttnThreads];
+    __shared__ float totals[kAttnThreads];
+    const int seq = blockIdx.x / sp.tiles_per_seq, tile = blockIdx.x - seq * sp.tiles_per_seq, tid = threadIdx.x;
+    int64_t before = 0, total = 0, in;
+    int s;
+    auto units = [&](int b) -> int64_t {
+        const int64_t n = (int64_t)SplitRange<STEP>(a, b).steps * sp.tiles_per_seq;
+        if (b < seq) before += n;
+        return n;
+    };
+    locate_unit<kAttnThreads>(a.pages.n_seqs, [](int64_t) { return int64_t(-1); }, units, located, s, in, total);
+    // (Each thread counted its own sequences: the ones before this are summed over the block.)
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) before += __shfl_xor(before, d);
+    __syncthreads();
+    if (tid % kWave == 0) located.wave_sum[tid / kWave] = before;
+    __syncthreads();
+    before = 0;
+    for (int w = 0; w < kAttnThreads / kWave; ++w) before += located.wave_sum[w];
+    const uint32_t steps = SplitRange<STEP>(a, seq).steps;
+    const int64_t u0 = before + (int64_t)tile * steps, u1 = u0 + steps, shares = share_count(total, sp.shares);
+    const int64_t g0 = share_of(u0, total, shares), g1 = share_of(u1 - 1, total, shares);
+    if (g0 == g1) return;
+    const bool whole_first = share_start(g0, total, shares) == u0;
+    auto row_of = [&](int64_t g, int c) { return (size_t)(2 * g + (g == g0 && !whole_first ? 1 : 0)) * (size_t)sp.cols + c; };
+
+    const int tiles_per_head = sp.tiles_per_seq / a.pages.n_kv;
+    const int h = tile / tiles_per_head, first = 16 * (tile - h * tiles_per_head);
+    const int n_cols = a.group - first < 16 ? a.group - first : 16;
+    const int lanes = a.head_dim / 4;  // threads of a column
+    const float* ml = sp.part + 2 * (size_t)sp.shares * (size_t)sp.cols * (size_t)a.head_dim;
+    // A column's parts over as many threads as there are: `ways` per 4 channels.
+    for (int c0 = 0; c0 < n_cols;) {
+        int at_once = kAttnThreads / lanes;
+        if (at_once > n_cols - c0) at_once = n_cols - c0;
+        const int ways = kAttnThreads / (lanes * at_once);
+        const int way = tid / (lanes * at_once), rest = tid - way * (lanes * at_once), c = c0 + rest / lanes, x = 4 * (rest % lanes);
+        float top = kNegInf, l = 0.0f;
+        f32x4 sum = {0, 0, 0, 0};
+        if (way < ways) {
+            for (int64_t g = g0 + way; g <= g1; g += ways) top = fmaxf(top, ml[2 * row_of(g, c)]);
+            const float ref = top == kNegInf ? 0.0f : top;
+            for (int64_t g = g0 + way; g <= g1; g += ways) {
+                const size_t row = row_of(g, c);
+                const float f = exp2_hw(ml[2 * row] - ref);
+                const f32x4 part = *reinterpret_cast<const f32x4*>(sp.part + row * (size_t)a.head_dim + x);
+                l = __builtin_fmaf(ml[2 * row + 1], f, l);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(part[i], f, sum[i]);
+            }
+        }
+        __shared__ float tops[kAttnThreads];
+        __syncthreads();
+        sums[tid] = sum;
+        totals[tid] = l;
+        tops[tid] = top;
+        __syncthreads();
+        if (way == 0) {
+            float all = kNegInf;
+            for (int w = 0; w < ways; ++w) all = fmaxf(all, tops[w * lanes * at_once + rest]);
+            l = 0.0f;
+            sum = f32x4{0, 0, 0, 0};
+            for (int w = 0; w < ways; ++w) {
+                const int i = w * lanes * at_once + rest;
+                const float f = tops[i] == kNegInf ? 0.0f : exp2_hw(tops[i] - all);
+                l = __builtin_fmaf(totals[i], f, l);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) sum[y] = __builtin_fmaf(sums[i][y], f, sum[y]);
+            }
+            const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] = l == 0.0f ? 0.0f : sum[i] * f;
+            const size_t row = (size_t)seq * (size_t)a.nq + (size_t)(h * a.group + first + c);
+            store4_from_f32(a.out, a.dtype, row * (size_t)a.head_dim + x, sum);
+        }
+        c0 += at_once;
+    }
 }
 
 // The kernel of a cache type, the narrowest that holds head_dim.

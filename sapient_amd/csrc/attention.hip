@@ -58,6 +58,46 @@ int dispatch_tiles(const AttnArgs& a, int cache_dtype, int64_t blocks, int tiles
     });
 }
 
+// Shares of a call's single tokens: as many blocks as the GPU holds at once, or the most units there can be.
+struct SplitPlan {
+    int tiles, cols, shares;
+    int64_t bytes;
+};
+SplitPlan split_plan(int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages, int64_t page_size, int64_t head_dim) {
+    SplitPlan p;
+    const int64_t group = nq / nkv;
+    const int64_t tiles = (group + 15) / 16 * nkv;
+    const int64_t steps = max_pages * page_size / 64 + 1;  // the smaller of the kernels' steps
+    int64_t shares = 256 * (head_dim > 128 ? 1 : 2);
+    if ((__int128)n_seqs * tiles * steps < shares) shares = n_seqs * tiles * steps;
+    p.tiles = (int)tiles;
+    p.cols = (int)(group < 16 ? group : 16);
+    p.shares = (int)shares;
+    p.bytes = 2 * shares * p.cols * (head_dim + 2) * 4;
+    return p;
+}
+
+template <typename TC, bool HIGH>
+int launch_split(const AttnArgs& a, const SplitPlan& p, float* ws, hipStream_t s) {
+    return with_tile_kernel<TC, HIGH>(a.head_dim, [&](auto k) {
+        using K = decltype(k);
+        const SplitArgs sp{p.tiles, p.cols, p.shares, ws};
+        const int st = launch(paged_split_kernel<K>, dim3((unsigned)p.shares), kAttnThreads, s, a, sp);
+        if (st != SPH_OK) return st;
+        return launch(paged_join_kernel<K::kStep>, dim3((unsigned)(a.pages.n_seqs * p.tiles)), kAttnThreads, s, a, sp);
+    });
+}
+
+int dispatch_split(const AttnArgs& a, int cache_dtype, const SplitPlan& p, float* ws, hipStream_t s) {
+    return with_float_type(cache_dtype, [&](auto tc) -> int {
+        using TC = decltype(tc);
+        if constexpr (!__is_same(TC, float)) {
+            if (a.dtype == cache_dtype) return launch_split<TC, false>(a, p, ws, s);
+        }
+        return launch_split<TC, true>(a, p, ws, s);
+    });
+}
+
 }  // namespace
 }  // namespace sph
 
@@ -74,8 +114,10 @@ extern "C" int sph_paged_attention(const void* q, void* out, int64_t n_q_heads, 
                              nullptr, bad_page_flag);
     if (st != SPH_OK) return st;
     if (n_seqs == 0) return SPH_OK;
-    const int tiles = (a.group + 15) / 16;
-    return dispatch_tiles(a, cache_dtype, n_seqs * n_kv_heads * tiles, tiles, static_cast<hipStream_t>(stream));
+    const SplitPlan p = split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim);
+    if (n_seqs * (int64_t)p.tiles * kAttnThreads > UINT32_MAX) return SPH_EINVAL;
+    if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < p.bytes) return SPH_EINVAL;
+    return dispatch_split(a, cache_dtype, p, static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
 }
 
 extern "C" int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype,
@@ -103,7 +145,10 @@ extern "C" int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_h
 
 extern "C" int64_t sph_paged_attention_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_pages,
                                                  int64_t page_size, int64_t head_dim) {
-    return 0;
+    if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads != 0 || n_seqs < 0 || max_pages < 0 || page_size < 1 ||
+        head_dim < 1 || head_dim > 256)
+        return SPH_EINVAL;
+    return sph::split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim).bytes;
 }
 
 extern "C" int64_t sph_paged_attention_chunk_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs,

@@ -34,6 +34,7 @@ struct PagedTable {
     const int32_t* cu;     // [n_seqs + 1] or null: one new token per sequence
     int n_seqs, max_pages, n_pages, n_kv;
     Divisor page;  // by the page's tokens
+    int capacity;  // tokens that a row of the table has entries for
 
     // Pool row of token t (kv head 0; head h's is h · page_size further), or kNoRow.
     __device__ __forceinline__ uint32_t row(int seq, uint32_t t) const {
@@ -41,6 +42,14 @@ struct PagedTable {
         if (p >= (uint32_t)max_pages) return kNoRow;
         const uint32_t id = (uint32_t)table[(size_t)seq * (size_t)max_pages + p];
         return id < (uint32_t)n_pages ? id * (uint32_t)n_kv * page.d + (t - p * page.d) : kNoRow;
+    }
+
+    // Keys of sequence b that the table can name: its length, cut at the capacity (and then flagged, by one lane).
+    __device__ __forceinline__ int keys(int b, int32_t* bad, bool tell) const {
+        const int len = lens[b];
+        if (len <= capacity) return len < 0 ? 0 : len;
+        if (bad != nullptr && tell) *bad = 1;
+        return capacity;
     }
 
     // The rows [begin, end) of sequence b's new tokens among n_rows, whatever cu holds.
@@ -79,6 +88,8 @@ inline PagedTable paged_table(const int32_t* seq_lens, const int32_t* cu_q, cons
     p.n_pages = (int)n_pages;
     p.n_kv = (int)n_kv;
     p.page = Divisor((uint32_t)page_size);
+    const int64_t capacity = max_pages * page_size;
+    p.capacity = capacity < INT32_MAX ? (int)capacity : INT32_MAX;
     return p;
 }
 

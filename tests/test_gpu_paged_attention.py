@@ -90,3 +90,13 @@ def test_prefix(dev, types, window):
     say("prefix", types, window)
     got = ops.paged_attention_chunk(*c.to(dev), window=window, prefix_lens=torch.tensor(prefix, dtype=torch.int32, device=dev))
     check(got, c, "prefix", weights(dt, ct, True), window=window, prefix=prefix)
+
+
+def test_a_used_workspace_leaves_nothing(dev):
+    """What an earlier call, or anything, left in the workspace does not reach a result."""
+    for lens in ([333], [1, 333, 0, 16, 129], [700, 3, 650] * 5):
+        c = Batch(14, 2, 64, lens=lens, seed=7)
+        n = ops.paged_attention_workspace(14, 2, len(lens), c.table.shape[1], 16, 64)
+        ws = torch.full((n // 4 + 1,), float("nan"), device=dev).view(torch.uint8)
+        say("workspace", lens[:5])
+        check(ops.paged_attention(*c.to(dev), workspace=ws), c, "workspace", weights(F16, F16, False))
