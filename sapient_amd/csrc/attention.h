@@ -95,7 +95,8 @@ __device__ __forceinline__ void store4_from_f32(void* p, int dt, size_t i, f32x4
 }
 
 // Which sequence the unit pick(total) falls to, where sequence b has count(b) units, counted by the block's NT threads:
-// true, with the sequence and the unit's number within it, or false past the last. Every thread calls it.
+// true, with the sequence and the unit's number within it, or false where there is no such unit (negative, or past the
+// last). Every thread calls it.
 struct Located {
     int64_t wave_sum[kAttnThreads / kWave];
     int64_t within;
@@ -131,7 +132,7 @@ __device__ __forceinline__ bool locate_unit(int n_seqs, P pick, F count, Located
         sm.within = u - before;
     }
     __syncthreads();
-    if (u >= total) return false;
+    if (u < 0 || u >= total) return false;
     seq = sm.seq;
     within = sm.within;
     return true;
@@ -478,58 +479,130 @@ struct TileKernel {
     }
 };
 
-// The keys that any column of the tile may see, [lo, hi).
-__device__ __forceinline__ void key_range(const AttnArgs& a, const Tile& t, int keys, uint32_t& lo, uint32_t& hi) {
-    const int last_col = t.first + 15 < t.rows ? t.first + 15 : t.rows - 1;
+// ─────────────────────────────── chunks ───────────────────────────────
+// A chunk call's blocks take (sequence, tile of rows, kv head), and, where these are fewer than the GPU holds, equal
+// parts of the tile's keys, which paged_chunk_join_kernel sums. Which sequences the tiles belong to follows from cu_q
+// on the device: the grid has the most tiles there can be.
+struct ChunkSplit {
+    int splits;
+    float* part;  // [splits][n_rows · nq][head_dim] sums, then [splits][n_rows · nq][2] m and l
+};
+struct ChunkPart {
+    int split;
+    uint32_t lo, hi;      // the keys
+    uint32_t start, end;  // their steps, aligned
+};
+
+__device__ __forceinline__ void chunk_part_sum(const AttnArgs& a, const ChunkSplit& sp, int split, size_t q_row, int d, f32x4 sum) {
+    const size_t row = (size_t)split * (size_t)a.n_rows * (size_t)a.nq + q_row;
+    *reinterpret_cast<f32x4*>(sp.part + row * (size_t)a.head_dim + d) = sum;
+}
+__device__ __forceinline__ void chunk_part_ml(const AttnArgs& a, const ChunkSplit& sp, int split, size_t q_row, float m, float l) {
+    const size_t all = (size_t)a.n_rows * (size_t)a.nq, row = (size_t)split * all + q_row;
+    float* ml = sp.part + (size_t)sp.splits * all * (size_t)a.head_dim + 2 * row;
+    ml[0] = m;
+    ml[1] = l;
+}
+
+// The block's tile of ROWS rows and its part of the keys, in steps of KEYS; false where there is none. kv heads vary
+// fastest, so that with 8 of them each XCD keeps one's keys in its L2; of a sequence's tiles the last, with the most
+// keys, come first.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool chunk_tile(const AttnArgs& a, const ChunkSplit& sp, Located& sm, Tile& t, ChunkPart& part) {
+    const int n_kv = a.pages.n_kv;
+    uint32_t block = blockIdx.x;
+    t.h = (int)(block % (uint32_t)n_kv);
+    block /= (uint32_t)n_kv;
+    part.split = (int)(block % (uint32_t)sp.splits);
+    block /= (uint32_t)sp.splits;
+    auto tiles = [&](int b) -> int64_t {
+        int lo, hi;
+        a.pages.new_rows(b, a.n_rows, lo, hi);
+        return ((int64_t)(hi - lo) * a.group + ROWS - 1) / ROWS;
+    };
+    int64_t total, tile;
+    if (!locate_unit<kAttnThreads>(a.pages.n_seqs, [&](int64_t n) { return n - 1 - (int64_t)block; }, tiles, sm, t.seq, tile, total))
+        return false;
+    int begin, end;
+    a.pages.new_rows(t.seq, a.n_rows, begin, end);
+    t.row0 = begin;
+    t.rows = (end - begin) * a.group;
+    t.first = ROWS * (int)tile;
+    t.pos0 = a.pages.lens[t.seq] - (end - begin);
+    if (t.pos0 < 0 && threadIdx.x == 0 && a.bad != nullptr) *a.bad = 1;
+    const int keys = a.pages.keys(t.seq, a.bad, threadIdx.x == 0);
+
+    // The keys that any of the tile's rows may see.
+    const int last_col = t.first + ROWS - 1 < t.rows ? t.first + ROWS - 1 : t.rows - 1;
     const int pos_first = t.pos0 + t.first / a.group, pos_last = t.pos0 + last_col / a.group;
     const int prefix = a.prefix != nullptr ? a.prefix[t.seq] : 0;
-    int end = pos_last + 1 > prefix ? pos_last + 1 : prefix;
-    if (pos_last < 0) end = 0;
-    if (end > keys) end = keys;
-    int begin = a.window > 0 && pos_first - a.window + 1 > 0 ? pos_first - a.window + 1 : 0;
-    hi = end < 0 ? 0u : (uint32_t)end;
-    lo = (uint32_t)begin < hi ? (uint32_t)begin : hi;
+    int to = pos_last + 1 > prefix ? pos_last + 1 : prefix;
+    if (to > keys) to = keys;
+    if (pos_last < 0) to = 0;
+    const int from = a.window > 0 && pos_first - a.window + 1 > 0 ? pos_first - a.window + 1 : 0;
+    part.hi = (uint32_t)to;
+    part.lo = from < to ? (uint32_t)from : part.hi;
+    const uint32_t start = part.lo & ~(uint32_t)(KEYS - 1), steps = (part.hi - start + KEYS - 1) / KEYS;
+    const uint32_t each = (steps + sp.splits - 1) / sp.splits;
+    part.start = start + KEYS * each * part.split;
+    part.end = start + KEYS * (each * (part.split + 1) < steps ? each * (part.split + 1) : steps);
+    if (part.start > part.end) part.start = part.end;
+    return true;
 }
 
 template <typename K>
-__global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_tiles_kernel(AttnArgs a, int tiles_per_seq) {
+__global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_tiles_kernel(AttnArgs a, ChunkSplit sp) {
     __shared__ typename K::Shared sm;
-    const int n_kv = a.pages.n_kv;
     Tile t;
-    t.h = blockIdx.x % n_kv;
-    int64_t unit = blockIdx.x / n_kv;
-    int begin, end;
-    if (a.pages.cu == nullptr) {
-        t.seq = (int)(unit / tiles_per_seq);
-        unit -= (int64_t)t.seq * tiles_per_seq;
-        begin = t.seq;
-        end = begin + 1;
-    } else {
-        auto tiles = [&](int b) -> int64_t {
-            int lo, hi;
-            a.pages.new_rows(b, a.n_rows, lo, hi);
-            return ((int64_t)(hi - lo) * a.group + 15) / 16;
-        };
-        int64_t total;
-        if (!locate_unit<kAttnThreads>(a.pages.n_seqs, [&](int64_t) { return unit; }, tiles, sm.located, t.seq, unit, total)) return;
-        a.pages.new_rows(t.seq, a.n_rows, begin, end);
-    }
-    const int len = a.pages.lens[t.seq];
-    t.row0 = begin;
-    t.rows = (end - begin) * a.group;
-    t.first = 16 * (int)unit;
-    t.pos0 = len - (end - begin);
-    if (a.bad != nullptr && a.pages.cu != nullptr && t.pos0 < 0 && threadIdx.x == 0) *a.bad = 1;
-    uint32_t lo, hi;
-    key_range(a, t, a.pages.keys(t.seq, a.bad, threadIdx.x == 0), lo, hi);
+    ChunkPart part;
+    if (!chunk_tile<16, K::kStep>(a, sp, sm.located, t, part)) return;
+    const uint32_t lo = part.lo > part.start ? part.lo : part.start, hi = part.hi < part.end ? part.hi : part.end;
+    auto row_of = [&](int c) {
+        const int col = t.first + c, tok = col / a.group;
+        return (size_t)(t.row0 + tok) * (size_t)a.nq + (size_t)(t.h * a.group + (col - tok * a.group));
+    };
     K k;
-    k.attend(a, sm, t, lo, hi, [&](int c, int d, float, float total, f32x4 sum) {
-        const int col = t.first + c, tok = col / a.group, head = t.h * a.group + (col - tok * a.group);
-        const float f = total == 0.0f ? 0.0f : 1.0f / total;
+    if (sp.splits == 1) {
+        k.attend(a, sm, t, lo, hi, [&](int c, int d, float, float l, f32x4 sum) {
+            const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] = total == 0.0f ? 0.0f : sum[i] * f;
-        store4_from_f32(a.out, a.dtype, ((size_t)(t.row0 + tok) * (size_t)a.nq + (size_t)head) * (size_t)a.head_dim + d, sum);
-    });
+            for (int i = 0; i < 4; ++i) sum[i] = l == 0.0f ? 0.0f : sum[i] * f;
+            store4_from_f32(a.out, a.dtype, row_of(c) * (size_t)a.head_dim + d, sum);
+        });
+    } else {
+        k.attend(a, sm, t, lo, hi, [&](int c, int d, float m, float l, f32x4 sum) {
+            chunk_part_sum(a, sp, part.split, row_of(c), d, sum);
+            if (d == 0) chunk_part_ml(a, sp, part.split, row_of(c), m, l);
+        });
+    }
+}
+
+// 4 channels of a row a thread. Rows that are no tokens have no parts: cu_q's last entry says where they begin.
+__global__ __launch_bounds__(kAttnThreads) void paged_chunk_join_kernel(AttnArgs a, ChunkSplit sp) {
+    const size_t all = (size_t)a.n_rows * (size_t)a.nq;
+    const uint32_t lanes = (uint32_t)a.head_dim / 4;
+    const size_t i = (size_t)blockIdx.x * kAttnThreads + threadIdx.x, q_row = i / lanes;
+    const int x = 4 * (int)(i - q_row * lanes);
+    if (q_row >= all) return;
+    const int64_t row = (int64_t)(q_row / (size_t)a.nq);
+    if (row < a.pages.cu[0] || row >= a.pages.cu[a.pages.n_seqs]) return;
+    const float* ml = sp.part + (size_t)sp.splits * all * (size_t)a.head_dim + 2 * q_row;
+    float top = kNegInf;
+    for (int s = 0; s < sp.splits; ++s) top = fmaxf(top, ml[2 * s * all]);
+    const float ref = top == kNegInf ? 0.0f : top;
+    float l = 0.0f;
+    f32x4 sum = {0, 0, 0, 0};
+    for (int s = 0; s < sp.splits; ++s) {
+        const float f = exp2_hw(ml[2 * s * all] - ref);
+        const f32x4 p = *reinterpret_cast<const f32x4*>(sp.part + (s * all + q_row) * (size_t)a.head_dim + x);
+        l = __builtin_fmaf(ml[2 * s * all + 1], f, l);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] = __builtin_fmaf(p[c], f, sum[c]);
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum[c] = l == 0.0f ? 0.0f : sum[c] * f;
+    store4_from_f32(a.out, a.dtype, q_row * (size_t)a.head_dim + x, sum);
 }
 
 // ───────────────────────── single tokens, split ─────────────────────────

@@ -1,5 +1,5 @@
 // attention.hip — entry points of attention over the paged KV cache (kernels and their mathematics: attention.h).
-#include "attention.h"
+#include "attention_prompt.h"
 
 #include <math.h>
 
@@ -40,22 +40,48 @@ int attn_args(AttnArgs& a, const void* q, void* out, int64_t n_q_heads, int64_t 
 
 namespace {
 
-template <typename TC, bool HIGH>
-int launch_tiles(const AttnArgs& a, int64_t blocks, int tiles_per_seq, hipStream_t s) {
-    if (blocks * kAttnThreads > UINT32_MAX) return SPH_EINVAL;
-    return with_tile_kernel<TC, HIGH>(a.head_dim, [&](auto k) {
-        return launch(paged_tiles_kernel<decltype(k)>, dim3((unsigned)blocks), kAttnThreads, s, a, tiles_per_seq);
-    });
+// Parts of a chunk's keys, where its tiles alone are fewer than the blocks that the GPU holds: at most 16, of 512 keys or
+// more were the table full.
+struct ChunkPlan {
+    int64_t tiles;  // the most there can be, of one kv head: every sequence's end in at most one that is not full
+    int splits;
+    int64_t bytes;
+};
+ChunkPlan chunk_plan(int rows_per_tile, int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages, int64_t page_size,
+                     int64_t n_rows, int64_t head_dim) {
+    ChunkPlan p;
+    p.tiles = n_rows * (nq / nkv) / rows_per_tile + (n_seqs < n_rows ? n_seqs : n_rows);
+    const int64_t blocks = p.tiles * nkv, slots = 256 * (head_dim > 128 ? 1 : 2), most = max_pages * page_size / 512;
+    int64_t s = blocks > 0 ? slots / blocks : 1;
+    if (s > 16) s = 16;
+    if (s > most) s = most;
+    if (s < 1) s = 1;
+    p.splits = (int)s;
+    p.bytes = s > 1 ? s * n_rows * nq * (head_dim + 2) * 4 : 0;
+    return p;
 }
 
-int dispatch_tiles(const AttnArgs& a, int cache_dtype, int64_t blocks, int tiles_per_seq, hipStream_t s) {
-    return with_float_type(cache_dtype, [&](auto tc) -> int {
-        using TC = decltype(tc);
-        if constexpr (!__is_same(TC, float)) {
-            if (a.dtype == cache_dtype) return launch_tiles<TC, false>(a, blocks, tiles_per_seq, s);
-        }
-        return launch_tiles<TC, true>(a, blocks, tiles_per_seq, s);
+// Chunks of one half type take tiles of 128 rows, others of 16.
+inline int chunk_rows(bool prompt) { return prompt ? kPromptRows : 16; }
+
+template <typename TC, bool HIGH>
+int launch_tiles(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) {
+    return with_tile_kernel<TC, HIGH>(a.head_dim, [&](auto k) {
+        return launch(paged_tiles_kernel<decltype(k)>, dim3(blocks), kAttnThreads, s, a, sp);
     });
+}
+template <typename TC>
+int launch_prompt(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) {
+    auto go = [&](auto kernel) { return launch(kernel, dim3(blocks), kAttnThreads, s, a, sp); };
+    switch (a.head_dim) {
+    case 64: return go(paged_prompt_kernel<TC, 64, true>);
+    case 128: return go(paged_prompt_kernel<TC, 128, true>);
+    case 256: return go(paged_prompt_kernel<TC, 256, true>);
+    default:
+        return a.head_dim < 64    ? go(paged_prompt_kernel<TC, 64, false>)
+               : a.head_dim < 128 ? go(paged_prompt_kernel<TC, 128, false>)
+                                  : go(paged_prompt_kernel<TC, 256, false>);
+    }
 }
 
 // Shares of a call's single tokens: as many blocks as the GPU holds at once, or the most units there can be.
@@ -138,9 +164,23 @@ extern "C" int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_h
     const uintptr_t bytes = (uintptr_t)n_q_heads * (uintptr_t)n_tokens * (uintptr_t)head_dim * dtype_size(dtype);
     const uintptr_t x = (uintptr_t)q, y = (uintptr_t)out;
     if (x < y + bytes && y < x + bytes) return SPH_EINVAL;  // a row's columns are read by one block and written by another
-    // Every sequence's tiles end in at most one that is not full.
-    const int64_t tiles = n_tokens * a.group / 16 + n_seqs;
-    return dispatch_tiles(a, cache_dtype, tiles * n_kv_heads, 1, static_cast<hipStream_t>(stream));
+    const bool prompt = dtype == cache_dtype && dtype != SPH_F32;
+    const ChunkPlan p = chunk_plan(chunk_rows(prompt), n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, n_tokens, head_dim);
+    if (p.bytes > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < p.bytes)) return SPH_EINVAL;
+    const __int128 blocks = (__int128)p.tiles * n_kv_heads * p.splits;
+    if (blocks * kAttnThreads > UINT32_MAX) return SPH_EINVAL;
+    const ChunkSplit sp{p.splits, static_cast<float*>(workspace)};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const unsigned n = (unsigned)blocks;
+    int r;
+    if (prompt) {
+        r = dtype == SPH_F16 ? launch_prompt<f16>(a, n, sp, s) : launch_prompt<bf16>(a, n, sp, s);
+    } else {
+        r = with_float_type(cache_dtype, [&](auto tc) { return launch_tiles<decltype(tc), true>(a, n, sp, s); });
+    }
+    if (r != SPH_OK || p.splits == 1) return r;
+    const int64_t threads = n_tokens * n_q_heads * (head_dim / 4);
+    return launch(paged_chunk_join_kernel, dim3((unsigned)((threads + kAttnThreads - 1) / kAttnThreads)), kAttnThreads, s, a, sp);
 }
 
 extern "C" int64_t sph_paged_attention_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_pages,
@@ -154,5 +194,15 @@ extern "C" int64_t sph_paged_attention_workspace(int64_t n_q_heads, int64_t n_kv
 extern "C" int64_t sph_paged_attention_chunk_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs,
                                                        int64_t max_pages, int64_t page_size, int64_t n_tokens,
                                                        int64_t head_dim) {
-    return 0;
+    if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads != 0 || n_seqs < 0 || max_pages < 0 || page_size < 1 ||
+        head_dim < 1 || head_dim > 256 || n_tokens < 0)
+        return SPH_EINVAL;
+    // The larger of the two tiles' plans.
+    int64_t most = 0;
+    for (const bool prompt : {false, true}) {
+        const int64_t n = sph::chunk_plan(sph::chunk_rows(prompt), n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, n_tokens,
+                                          head_dim).bytes;
+        if (n > most) most = n;
+    }
+    return most;
 }

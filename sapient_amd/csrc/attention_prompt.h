@@ -1,0 +1,279 @@
+// attention_prompt.h — the kernel of chunks whose q and cache are one half type: 128 rows a block (mathematics and
+// the argument block: attention.h).
+//
+// Four waves of 32 columns (rows of q: tokens and the query heads of one kv head, so that a block reads its keys once
+// for the whole group) share steps of 64 keys through LDS, on 32x32x16 matrix instructions. Scores are transposed
+// (S^T = K Q^T) as in the 16-column kernel: lane (j = lane % 32, h = lane / 32) holds column j's scores of tokens 8b +
+// 4h + 0..3, which is the order in which it feeds them back as the second operand, so weights never leave their lane.
+// In LDS
+//  - K lies as it comes, rows of DP channels in 16-byte pieces, piece c of row r at c ^ (r & 7): the 8 rows that a
+//    quarter of a read touches are in 8 different groups of banks;
+//  - V lies transposed, 64 tokens a channel, 8 pieces of 8 tokens in the order of the weights' slots (tokens 16m +
+//    4h + 0..3 and 16m + 8 + 4h + 0..3 are piece 2m + h), piece c of channel d at c ^ ((d ^ d >> 3) & 7). A thread turns
+//    4 tokens by 8 channels with 16 v_perm_b32 on the way, once for the four waves.
+// Two buffers: the next step's rows are on their way into registers while this step is computed, and are written to
+// the other buffer after it; one barrier a step.
+#pragma once
+
+#include "attention.h"
+
+namespace sph {
+namespace {
+
+constexpr int kPromptRows = 128, kPromptKeys = 64;
+
+template <typename TC>
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (__is_same(TC, f16))
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+template <typename TC, int DP>
+struct PromptShared {
+    alignas(16) uint16_t k[2][kPromptKeys * DP];
+    alignas(16) uint16_t v[2][kPromptKeys * DP];
+    Located located;
+};
+
+// EXACT: head_dim is DP.
+template <typename TC, int DP, bool EXACT>
+__global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_kernel(AttnArgs a, ChunkSplit sp) {
+    __shared__ PromptShared<TC, DP> sm;
+    constexpr int KS = DP / 16;                    // k steps of a score
+    constexpr int DB = DP / 32;                    // blocks of channels
+    constexpr int CH = DP / 8;                     // 16-byte pieces of a row
+    constexpr int KL = kPromptKeys * CH / kAttnThreads;  // pieces of K per thread and step
+    constexpr int VE = DP == 64 ? 4 : 8;           // channels of V that a thread turns
+    constexpr int VU = 16 * (DP / VE) / kAttnThreads;
+    constexpr int VW = VE / 2;
+    constexpr float kLift = __is_same(TC, f16) ? 7.0f : 0.0f;
+    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, j = lane % 32, h = lane / 32;
+    const int D = EXACT ? DP : a.head_dim;
+
+    Tile t;
+    ChunkPart part;
+    if (!chunk_tile<kPromptRows, kPromptKeys>(a, sp, sm.located, t, part)) return;
+    const uint32_t lo = part.lo, hi = part.hi;
+
+    // This lane's column, and the positions of the wave's.
+    const int wave_first = t.first + 32 * wave;
+    const int n_cols = t.rows - wave_first < 32 ? t.rows - wave_first : 32;  // may be 0 and less
+    const int col = wave_first + j < t.rows ? wave_first + j : t.rows - 1;
+    const int tok = col / a.group, head = t.h * a.group + (col - tok * a.group), pos = t.pos0 + tok;
+    const int pos_first = t.pos0 + wave_first / a.group;
+    const int pos_last = t.pos0 + (wave_first + (n_cols > 0 ? n_cols : 1) - 1) / a.group;
+    const int prefix = a.prefix != nullptr ? a.prefix[t.seq] : 0;
+    const float slope = a.slopes != nullptr ? a.slopes[head] : 0.0f;
+    const size_t q_row = (size_t)(t.row0 + tok) * (size_t)a.nq + (size_t)head;
+
+    u32x4 q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const int d = 16 * s + 8 * h;
+        q[s] = u32x4{0, 0, 0, 0};
+        if (EXACT || d < D) q[s] = *reinterpret_cast<const u32x4*>(static_cast<const TC*>(a.q) + q_row * (size_t)D + d);
+    }
+
+    const TC *kc = static_cast<const TC*>(a.kc), *vc = static_cast<const TC*>(a.vc);
+    const uint32_t head_rows = (uint32_t)t.h * a.pages.page.d;
+    auto row_at = [&](uint32_t t0) -> uint32_t {  // the pool row of key t0 + lane
+        const uint32_t k = t0 + (uint32_t)lane;
+        if (k < lo || k >= hi) return kNoRow;
+        const uint32_t r = a.pages.row(t.seq, k);
+        if (r == kNoRow) {
+            if (a.bad != nullptr) *a.bad = 1;
+            return kNoRow;
+        }
+        return r + head_rows;
+    };
+    // This thread's part of a step's K and V, as it comes from memory. Row 0 stands in for a missing K row (its
+    // scores are masked); a missing V row is zeros, since 0 · inf is not 0.
+    u32x4 kr[KL];
+    uint32_t vr[VU][4][VW];
+    const int v_oct = (tid & 7) | ((tid >> 4) & 1) << 3, v_quad = ((tid >> 3) & 1) << 1 | ((tid >> 5) & 1) | (tid >> 6) << 2;
+    auto load_step = [&](uint32_t rows) {
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+            const int piece = i * kAttnThreads + tid, row = piece / CH, d = 8 * (piece % CH);
+            const uint32_t r = __shfl(rows, row);
+            kr[i] = u32x4{0, 0, 0, 0};
+            if (EXACT || d < D) kr[i] = *reinterpret_cast<const u32x4*>(kc + (size_t)(r == kNoRow ? 0u : r) * (size_t)D + d);
+        }
+#pragma unroll
+        for (int u = 0; u < VU; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t r = __shfl(rows, 4 * v_quad + e);
+                const int d = VE * (v_oct + 16 * u);
+#pragma unroll
+                for (int w = 0; w < VW; ++w) vr[u][e][w] = 0u;
+                if (r != kNoRow && (EXACT || d < D)) {
+                    const TC* p = vc + (size_t)r * (size_t)D + d;
+                    if constexpr (VW == 4) {
+                        const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) vr[u][e][w] = x[w];
+                    } else {
+                        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+                        vr[u][e][0] = x[0];
+                        vr[u][e][1] = x[1];
+                    }
+                }
+            }
+    };
+    auto store_step = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+            const int piece = i * kAttnThreads + tid, row = piece / CH, c = piece % CH;
+            *reinterpret_cast<u32x4*>(&sm.k[buf][row * DP + 8 * (c ^ (row & 7))]) = kr[i];
+        }
+#pragma unroll
+        for (int u = 0; u < VU; ++u)
+#pragma unroll
+            for (int n = 0; n < VE; ++n) {
+                const int d = VE * (v_oct + 16 * u) + n;
+                const uint32_t sel = n % 2 ? 0x07060302u : 0x05040100u;
+                const u32x2 x = {__builtin_amdgcn_perm(vr[u][1][n / 2], vr[u][0][n / 2], sel),
+                                 __builtin_amdgcn_perm(vr[u][3][n / 2], vr[u][2][n / 2], sel)};
+                const int piece = 2 * (v_quad / 4) + (v_quad & 1), half = (v_quad >> 1) & 1;
+                *reinterpret_cast<u32x2*>(&sm.v[buf][d * kPromptKeys + 8 * (piece ^ ((d ^ d >> 3) & 7)) + 4 * half]) = x;
+            }
+    };
+
+    float m = kNegInf, l = 0.0f;
+    f32x16 acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
+
+    const bool plain = a.cap == 0.0f && a.slopes == nullptr && a.scale > 0.0f;
+    const float unit = plain ? a.scale * kLog2e : 1.0f;  // scores to log2 units, where nothing has to be done to them
+
+    uint32_t t0 = part.start;
+    const uint32_t end = part.end;  // steps [start, end) of 64 keys
+    uint32_t rows = row_at(t0), rows_next = row_at(t0 + kPromptKeys);
+    if (t0 < end) {
+        load_step(rows);
+        store_step(0);
+    }
+    __syncthreads();
+    for (int buf = 0; t0 < end; t0 += kPromptKeys, buf ^= 1) {
+        const bool more = t0 + kPromptKeys < end;
+        const uint32_t rows_after = row_at(t0 + 2 * kPromptKeys);
+        if (more) load_step(rows_next);
+
+        const uint64_t there = __ballot(rows != kNoRow);
+        const int last = (int)t0 + kPromptKeys - 1;
+        const bool none = n_cols <= 0 || (pos_last < (int)t0 && prefix <= (int)t0) ||
+                          (a.window > 0 && pos_first - last >= a.window);
+        if (!none) {
+            f32x16 s[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < KS; ++c) {
+                    const int row = 32 * b + j;
+                    const u32x4 k = *reinterpret_cast<const u32x4*>(&sm.k[buf][row * DP + 8 * ((2 * c + h) ^ (row & 7))]);
+                    s[b] = mma32<TC>(k, q[c], s[b]);
+                }
+            }
+            const bool seen = there == ~uint64_t(0) && pos_first >= 0 && (last <= pos_first || last < prefix) &&
+                              (a.window == 0 || pos_last - (int)t0 < a.window);
+            if (!plain) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        float x = s[b][r] * a.scale;
+                        if (a.cap != 0.0f) x = a.cap * score_tanh<false>(x / a.cap);
+                        if (a.slopes != nullptr) x -= slope * fabsf((float)(pos - ((int)t0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4)));
+                        s[b][r] = x * kLog2e;
+                    }
+            }
+            if (!seen) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int i = 32 * b + 8 * (r / 4) + 4 * h + r % 4, p = (int)t0 + i;
+                        const bool see = ((there >> i) & 1) && pos >= 0 && (p <= pos || p < prefix) &&
+                                         (a.window == 0 || pos - p < a.window);
+                        if (!see) s[b][r] = kNegInf;
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+            top *= unit;
+            if (__any(top > m + (kLift + kSlack))) {
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float m_new = fmaxf(m, top - kLift);
+                const float f = m_new == kNegInf ? 1.0f : exp2_hw(m - m_new);
+                m = m_new;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+            }
+            const float ref = m == kNegInf ? 0.0f : m;
+            u32x4 p[4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const float x = exp2_hw(__builtin_fmaf(s[b][r], unit, -ref)), y = exp2_hw(__builtin_fmaf(s[b][r + 1], unit, -ref));
+                    l += x + y;
+                    p[2 * b + r / 8][r % 8 / 2] = narrow2<TC>(x, y);
+                }
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int ch = 32 * d + j;
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(
+                        &sm.v[buf][ch * kPromptKeys + 8 * ((2 * i + h) ^ ((ch ^ ch >> 3) & 7))]);
+                    acc[d] = mma32<TC>(v, p[i], acc[d]);
+                }
+        }
+        if (more) store_step(buf ^ 1);
+        rows = rows_next;
+        rows_next = rows_after;
+        __syncthreads();
+    }
+
+    l += __shfl_xor(l, 32);
+    if (j >= n_cols) return;
+    if (sp.splits == 1) {
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int ch = 32 * d + 2 * r + 4 * h;
+                f32x4 o;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : acc[d][r + i] * f;
+                if (EXACT || ch < D) store4_from_f32(a.out, a.dtype, q_row * (size_t)D + ch, o);
+            }
+    } else {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int ch = 32 * d + 2 * r + 4 * h;
+                if (EXACT || ch < D) chunk_part_sum(a, sp, part.split, q_row, ch, f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]});
+            }
+        if (h == 0) chunk_part_ml(a, sp, part.split, q_row, m, l);
+    }
+}
+
+}  // namespace
+}  // namespace sph
