@@ -138,6 +138,14 @@ __device__ __forceinline__ bool locate_unit(int n_seqs, P pick, F count, Located
     return true;
 }
 
+// Of the keys t0 .. t0 + 63, those in `there` that a row at position pos sees, as bits.
+__device__ __forceinline__ uint64_t visible(uint64_t there, int t0, int pos, int prefix, int window) {
+    auto below = [](int n) { return n >= 64 ? ~uint64_t(0) : n <= 0 ? uint64_t(0) : (uint64_t(1) << n) - 1; };
+    uint64_t see = below(pos - t0 + 1) | below(prefix - t0);
+    if (window > 0) see &= ~below(pos - window + 1 - t0);
+    return pos < 0 ? 0 : see & there;
+}
+
 // A tile's 16 columns: the rows (token i of the sequence's new ones, head h · group + c) with number i · group + c in
 // [first, first + 16) of `rows`, for kv head h.
 struct Tile {
@@ -193,6 +201,7 @@ struct TileKernel {
         const int pos_first = t.pos0 + t.first / a.group, pos_last = t.pos0 + (t.first + n_cols - 1) / a.group;
         const int prefix = a.prefix != nullptr ? a.prefix[t.seq] : 0;
         const float slope = a.slopes != nullptr ? a.slopes[head] : 0.0f;
+        const float inv_cap = a.cap != 0.0f ? 1.0f / a.cap : 0.0f;
 
         // q, as the B operand: column j, channels of this lane's k slots.
         float unit = a.scale;
@@ -349,21 +358,17 @@ struct TileKernel {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float x = s[b][r] * unit;
-                        if (a.cap != 0.0f) x = a.cap * score_tanh<HIGH || kF32>(x / a.cap);
+                        if (a.cap != 0.0f) x = a.cap * score_tanh<HIGH || kF32>(x * inv_cap);
                         if (a.slopes != nullptr) x -= slope * fabsf((float)(pos - (int)(t0 + 16 * b + 4 * g + r)));
                         s[b][r] = x * kLog2e;
                     }
             }
             if (!seen) {
+                const uint32_t see = (uint32_t)visible(there, (int)t0, pos, prefix, a.window) >> (4 * g);
 #pragma unroll
                 for (int b = 0; b < KB; ++b)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = 16 * b + 4 * g + r, p = (int)t0 + i;
-                        const bool see = ((there >> i) & 1) && pos >= 0 && (p <= pos || p < prefix) &&
-                                         (a.window == 0 || pos - p < a.window);
-                        if (!see) s[b][r] = kNegInf;
-                    }
+                    for (int r = 0; r < 4; ++r) s[b][r] = see & (1u << (16 * b + r)) ? s[b][r] : kNegInf;
             }
             if (!whole) {  // what lies in a row that is no key of the sequence may be anything, and 0 · inf is not 0
 #pragma unroll

@@ -88,8 +88,8 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
         }
         return r + head_rows;
     };
-    // This thread's part of a step's K and V, as it comes from memory. Row 0 stands in for a missing K row (its
-    // scores are masked); a missing V row is zeros, since 0 · inf is not 0.
+    // This thread's part of a step's K and V, as it comes from memory. Row 0 stands in for a missing one: its scores
+    // are masked, and as V it is cleared on the way to LDS, since 0 · inf is not 0.
     u32x4 kr[KL];
     uint32_t vr[VU][4][VW];
     const int v_oct = (tid & 7) | ((tid >> 4) & 1) << 3, v_quad = ((tid >> 3) & 1) << 1 | ((tid >> 5) & 1) | (tid >> 6) << 2;
@@ -109,8 +109,8 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
                 const int d = VE * (v_oct + 16 * u);
 #pragma unroll
                 for (int w = 0; w < VW; ++w) vr[u][e][w] = 0u;
-                if (r != kNoRow && (EXACT || d < D)) {
-                    const TC* p = vc + (size_t)r * (size_t)D + d;
+                if (EXACT || d < D) {
+                    const TC* p = vc + (size_t)(r == kNoRow ? 0u : r) * (size_t)D + d;
                     if constexpr (VW == 4) {
                         const u32x4 x = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
@@ -123,7 +123,17 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
                 }
             }
     };
-    auto store_step = [&](int buf) {
+    auto store_step = [&](int buf, uint64_t there) {
+        if (there != ~uint64_t(0)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!((there >> (4 * v_quad + e)) & 1)) {
+#pragma unroll
+                    for (int u = 0; u < VU; ++u)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vr[u][e][w] = 0u;
+                }
+        }
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int piece = i * kAttnThreads + tid, row = piece / CH, c = piece % CH;
@@ -150,6 +160,7 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
 
     const bool plain = a.cap == 0.0f && a.slopes == nullptr && a.scale > 0.0f;
+    const float inv_cap = a.cap != 0.0f ? 1.0f / a.cap : 0.0f;
     const float unit = plain ? a.scale * kLog2e : 1.0f;  // scores to log2 units, where nothing has to be done to them
 
     uint32_t t0 = part.start;
@@ -157,7 +168,7 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
     uint32_t rows = row_at(t0), rows_next = row_at(t0 + kPromptKeys);
     if (t0 < end) {
         load_step(rows);
-        store_step(0);
+        store_step(0, __ballot(rows != kNoRow));
     }
     __syncthreads();
     for (int buf = 0; t0 < end; t0 += kPromptKeys, buf ^= 1) {
@@ -172,16 +183,18 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
         if (!none) {
             f32x16 s[2];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+            // (Two chains of products side by side: each waits for its own last one.)
 #pragma unroll
-                for (int c = 0; c < KS; ++c) {
+            for (int c = 0; c < KS; ++c)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
                     const int row = 32 * b + j;
                     const u32x4 k = *reinterpret_cast<const u32x4*>(&sm.k[buf][row * DP + 8 * ((2 * c + h) ^ (row & 7))]);
                     s[b] = mma32<TC>(k, q[c], s[b]);
                 }
-            }
             const bool seen = there == ~uint64_t(0) && pos_first >= 0 && (last <= pos_first || last < prefix) &&
                               (a.window == 0 || pos_last - (int)t0 < a.window);
             if (!plain) {
@@ -190,21 +203,18 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         float x = s[b][r] * a.scale;
-                        if (a.cap != 0.0f) x = a.cap * score_tanh<false>(x / a.cap);
+                        if (a.cap != 0.0f) x = a.cap * score_tanh<false>(x * inv_cap);
                         if (a.slopes != nullptr) x -= slope * fabsf((float)(pos - ((int)t0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4)));
                         s[b][r] = x * kLog2e;
                     }
             }
             if (!seen) {
+                const uint64_t see = visible(there, (int)t0, pos, prefix, a.window) >> (4 * h);
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = 32 * b + 8 * (r / 4) + 4 * h + r % 4, p = (int)t0 + i;
-                        const bool see = ((there >> i) & 1) && pos >= 0 && (p <= pos || p < prefix) &&
-                                         (a.window == 0 || pos - p < a.window);
-                        if (!see) s[b][r] = kNegInf;
-                    }
+                    for (int r = 0; r < 16; ++r)
+                        s[b][r] = (uint32_t)(see >> (32 * b)) & (1u << (8 * (r / 4) + r % 4)) ? s[b][r] : kNegInf;
             }
             float top = s[0][0];
 #pragma unroll
@@ -234,16 +244,16 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
                     p[2 * b + r / 8][r % 8 / 2] = narrow2<TC>(x, y);
                 }
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int d = 0; d < DB; ++d) {
                     const int ch = 32 * d + j;
                     const u32x4 v = *reinterpret_cast<const u32x4*>(
                         &sm.v[buf][ch * kPromptKeys + 8 * ((2 * i + h) ^ ((ch ^ ch >> 3) & 7))]);
                     acc[d] = mma32<TC>(v, p[i], acc[d]);
                 }
         }
-        if (more) store_step(buf ^ 1);
+        if (more) store_step(buf ^ 1, __ballot(rows_next != kNoRow));
         rows = rows_next;
         rows_next = rows_after;
         __syncthreads();
