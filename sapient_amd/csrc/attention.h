@@ -254,23 +254,36 @@ struct TileKernel {
 
         const TC *kc = static_cast<const TC*>(a.kc), *vc = static_cast<const TC*>(a.vc);
         const uint32_t head_rows = (uint32_t)t.h * a.pages.page.d;
-        // Pool row of the step's token that this lane follows, or kNoRow outside [lo, hi) and where there is no page.
-        auto row_at = [&](uint32_t t0) -> uint32_t {
+        // The table's entry for the step's token that this lane follows, asked for two steps ahead (waiting for it where
+        // its rows' loads are made would wait for all loads before it), and the token's pool row, kNoRow past
+        // hi and where there is no page.
+        auto entry_at = [&](uint32_t t0) {
             const uint32_t k = t0 + (uint32_t)(lane % ST);
-            if (k < lo || k >= hi) return kNoRow;
-            const uint32_t r = a.pages.row(t.seq, k);
-            if (r == kNoRow) {
-                if (a.bad != nullptr) *a.bad = 1;
-                return kNoRow;
+            return a.pages.entry(t.seq, k < hi ? k : hi - 1);
+        };
+        auto row_at = [&](uint32_t t0, uint32_t id) -> uint32_t {
+            const uint32_t k = t0 + (uint32_t)(lane % ST);
+            const uint32_t r = a.pages.row_in(id, k < hi ? k : hi - 1);
+            if (k >= lo && k < hi && r == kNoRow && a.bad != nullptr) *a.bad = 1;
+            return k < hi && r != kNoRow ? r + head_rows : kNoRow;
+        };
+        // Where 16 neighbouring keys share a page, lanes find their rows from the block's first by an addition, not by an
+        // exchange through LDS.
+        const bool by_16 = a.pages.page.d % 16 == 0;
+        auto pool_row = [&](uint32_t rows, int block, int i) -> uint32_t {  // of the step's key 16 block + i
+            uint32_t r;
+            if (by_16) {
+                r = __builtin_amdgcn_readlane(rows, 16 * block);
+                return (r == kNoRow ? 0u : r) + (uint32_t)i;
             }
-            return r + head_rows;
+            r = __shfl(rows, 16 * block + i);
+            return r == kNoRow ? 0u : r;
         };
         // Row 0 stands in for a missing one: there to be read, and masked or cleared.
         auto load_k = [&](uint32_t rows, KRegs& k) {
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
-                const uint32_t r = __shfl(rows, 16 * b + j);
-                const TC* p = kc + (size_t)(r == kNoRow ? 0u : r) * (size_t)D;
+                const TC* p = kc + (size_t)pool_row(rows, b, j) * (size_t)D;
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     const int d = kF32 ? 16 * s + 4 * g : 32 * s + 8 * g;
@@ -282,8 +295,7 @@ struct TileKernel {
         auto load_v = [&](uint32_t rows, VRegs& v) {
 #pragma unroll
             for (int e = 0; e < VT; ++e) {
-                const uint32_t r = __shfl(rows, 16 * (e / 4) + 4 * g + e % 4);
-                const TC* p = vc + (size_t)(r == kNoRow ? 0u : r) * (size_t)D + E * j;
+                const TC* p = vc + (size_t)pool_row(rows, e / 4, 4 * g + e % 4) * (size_t)D + E * j;
                 constexpr int B = VW >= 4 ? 4 : 2;  // words per access
 #pragma unroll
                 for (int c = 0; c < VW / B; ++c) {
@@ -314,13 +326,19 @@ struct TileKernel {
         KRegs k;
         VRegs v;
         uint32_t t0 = (lo & ~(uint32_t)(ST - 1)) + (uint32_t)(wave * ST);
-        uint32_t rows = row_at(t0), rows_next = row_at(t0 + kStep);
-        if (t0 < hi) load_k(rows, k);
+        uint32_t rows = kNoRow, id_next = 0;
+        if (t0 < hi) {
+            const uint32_t id = entry_at(t0);
+            id_next = entry_at(t0 + kStep);
+            rows = row_at(t0, id);
+            load_k(rows, k);
+        }
         for (; t0 < hi; t0 += kStep) {
-            const uint32_t rows_after = row_at(t0 + 2 * kStep);
+            const uint32_t rows_next = row_at(t0 + kStep, id_next);
+            id_next = entry_at(t0 + 2 * kStep);
             load_v(rows, v);
             KRegs k_next;
-            if (t0 + kStep < hi) load_k(rows_next, k_next);
+            load_k(rows_next, k_next);  // (Past the end too: loads in a branch would all be waited for where any is.)
 
             f32x4 s[KB];
 #pragma unroll
@@ -341,7 +359,7 @@ struct TileKernel {
             }
 
             // Scores in log2 units, and the mask where the step is not all visible to all columns.
-            const uint32_t there = (uint32_t)__ballot(rows != kNoRow) & (uint32_t)((uint64_t(1) << ST) - 1);
+            const uint32_t there = (uint32_t)__ballot(rows != kNoRow && t0 + (uint32_t)(lane % ST) >= lo) & (uint32_t)((uint64_t(1) << ST) - 1);
             const bool whole = there == (uint32_t)((uint64_t(1) << ST) - 1);
             const uint32_t last = t0 + ST - 1;
             const bool seen = whole && pos_first >= 0 && ((int)last <= pos_first || (int)last < prefix) &&
@@ -433,7 +451,6 @@ struct TileKernel {
                 }
             }
             rows = rows_next;
-            rows_next = rows_after;
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -618,10 +635,14 @@ __global__ __launch_bounds__(kAttnThreads) void paged_chunk_join_kernel(AttnArgs
 // and the last can be part of one that other blocks share. Those go to the workspace, and paged_join_kernel sums
 // them in a fixed order. The shares follow the lengths on the device: nothing is read back, a captured call
 // serves any lengths.
+struct PartRange {
+    int first, count;  // slot of a tile's first part, and its parts; 0 where one share held the tile
+};
 struct SplitArgs {
     int tiles_per_seq;  // of 16 columns: (kv head, tile of its group)
     int cols;           // of the widest tile
     int shares;         // blocks
+    PartRange* ranges;  // [n_seqs · tiles_per_seq]
     float* part;        // [2 · shares][cols][head_dim] sums, then [2 · shares][cols][2] m and l
 };
 
@@ -675,6 +696,11 @@ __global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_split_ker
             uint32_t lo = r.start + step * K::kStep, hi = lo + n * K::kStep;
             if (lo < r.lo) lo = r.lo;
             if (hi > r.hi) hi = r.hi;
+            if (step == 0 && threadIdx.x == 0) {  // the share that begins a tile names its parts
+                const int64_t last = share_of(u + r.steps - 1, total, share_count(total, sp.shares));
+                sp.ranges[(size_t)seq * (size_t)sp.tiles_per_seq + tile] =
+                    PartRange{2 * share + (u == begin ? 0 : 1), n == r.steps ? 0 : (int)(last - share) + 1};
+            }
             K k;
             if (n == r.steps) {
                 k.attend(a, sm, t, lo, hi, [&](int c, int d, float, float l, f32x4 sum) {
@@ -702,87 +728,72 @@ __global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_split_ker
     }
 }
 
-// One block per (sequence, tile): nothing where one share held it, else the sum of its parts.
-template <int STEP>
+// One block per (sequence, query head): nothing where one share held its tile, else the sum of its parts, 4 channels a
+// thread and the parts over as many threads as that leaves.
 __global__ __launch_bounds__(kAttnThreads) void paged_join_kernel(AttnArgs a, SplitArgs sp) {
-    __shared__ Located located;
     __shared__ f32x4 sums[kAttnThreads];
-    __shared__ float totals[kAttnThreads];
-    const int seq = blockIdx.x / sp.tiles_per_seq, tile = blockIdx.x - seq * sp.tiles_per_seq, tid = threadIdx.x;
-    int64_t before = 0, total = 0, in;
-    int s;
-    auto units = [&](int b) -> int64_t {
-        const int64_t n = (int64_t)SplitRange<STEP>(a, b).steps * sp.tiles_per_seq;
-        if (b < seq) before += n;
-        return n;
-    };
-    locate_unit<kAttnThreads>(a.pages.n_seqs, [](int64_t) { return int64_t(-1); }, units, located, s, in, total);
-    // (Each thread counted its own sequences: the ones before this are summed over the block.)
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) before += __shfl_xor(before, d);
-    __syncthreads();
-    if (tid % kWave == 0) located.wave_sum[tid / kWave] = before;
-    __syncthreads();
-    before = 0;
-    for (int w = 0; w < kAttnThreads / kWave; ++w) before += located.wave_sum[w];
-    const uint32_t steps = SplitRange<STEP>(a, seq).steps;
-    const int64_t u0 = before + (int64_t)tile * steps, u1 = u0 + steps, shares = share_count(total, sp.shares);
-    const int64_t g0 = share_of(u0, total, shares), g1 = share_of(u1 - 1, total, shares);
-    if (g0 == g1) return;
-    const bool whole_first = share_start(g0, total, shares) == u0;
-    auto row_of = [&](int64_t g, int c) { return (size_t)(2 * g + (g == g0 && !whole_first ? 1 : 0)) * (size_t)sp.cols + c; };
-
-    const int tiles_per_head = sp.tiles_per_seq / a.pages.n_kv;
-    const int h = tile / tiles_per_head, first = 16 * (tile - h * tiles_per_head);
-    const int n_cols = a.group - first < 16 ? a.group - first : 16;
-    const int lanes = a.head_dim / 4;  // threads of a column
+    __shared__ float totals[kAttnThreads], tops[kAttnThreads];
+    const uint32_t q_row = blockIdx.x, tid = threadIdx.x;
+    const uint32_t seq = q_row / (uint32_t)a.nq, head = q_row - seq * (uint32_t)a.nq;
+    const uint32_t h = head / (uint32_t)a.group, in_group = head - h * (uint32_t)a.group;
+    const uint32_t tiles_per_head = (uint32_t)(sp.tiles_per_seq / a.pages.n_kv);
+    const PartRange range = sp.ranges[(size_t)seq * (size_t)sp.tiles_per_seq + h * tiles_per_head + in_group / 16];
+    if (range.count == 0) return;
+    const uint32_t c = in_group % 16, lanes = (uint32_t)a.head_dim / 4, ways = kAttnThreads / lanes, way = tid / lanes;
+    const uint32_t x = 4 * (tid - way * lanes);
+    // Part i of a tile is its first share's slot, then the first slots of the shares after it.
+    auto row_of = [&](int i) { return (size_t)(i == 0 ? range.first : (range.first & ~1) + 2 * i) * (size_t)sp.cols + c; };
     const float* ml = sp.part + 2 * (size_t)sp.shares * (size_t)sp.cols * (size_t)a.head_dim;
-    // A column's parts over as many threads as there are: `ways` per 4 channels.
-    for (int c0 = 0; c0 < n_cols;) {
-        int at_once = kAttnThreads / lanes;
-        if (at_once > n_cols - c0) at_once = n_cols - c0;
-        const int ways = kAttnThreads / (lanes * at_once);
-        const int way = tid / (lanes * at_once), rest = tid - way * (lanes * at_once), c = c0 + rest / lanes, x = 4 * (rest % lanes);
-        float top = kNegInf, l = 0.0f;
-        f32x4 sum = {0, 0, 0, 0};
-        if (way < ways) {
-            for (int64_t g = g0 + way; g <= g1; g += ways) top = fmaxf(top, ml[2 * row_of(g, c)]);
-            const float ref = top == kNegInf ? 0.0f : top;
-            for (int64_t g = g0 + way; g <= g1; g += ways) {
-                const size_t row = row_of(g, c);
-                const float f = exp2_hw(ml[2 * row] - ref);
-                const f32x4 part = *reinterpret_cast<const f32x4*>(sp.part + row * (size_t)a.head_dim + x);
-                l = __builtin_fmaf(ml[2 * row + 1], f, l);
+    float top = kNegInf, l = 0.0f;
+    f32x4 sum = {0, 0, 0, 0};
+    if (way < ways) {
+        // In groups of four, whose loads are in flight together.
+        for (int i0 = (int)way; i0 < range.count; i0 += 4 * (int)ways) {
+            float m4[4], l4[4];
+            f32x4 s4[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(part[i], f, sum[i]);
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * (int)ways;
+                const size_t row = row_of(i < range.count ? i : i0);
+                m4[k] = ml[2 * row];
+                l4[k] = ml[2 * row + 1];
+                s4[k] = *reinterpret_cast<const f32x4*>(sp.part + row * (size_t)a.head_dim + x);
+                if (i >= range.count) m4[k] = kNegInf;
             }
-        }
-        __shared__ float tops[kAttnThreads];
-        __syncthreads();
-        sums[tid] = sum;
-        totals[tid] = l;
-        tops[tid] = top;
-        __syncthreads();
-        if (way == 0) {
-            float all = kNegInf;
-            for (int w = 0; w < ways; ++w) all = fmaxf(all, tops[w * lanes * at_once + rest]);
-            l = 0.0f;
-            sum = f32x4{0, 0, 0, 0};
-            for (int w = 0; w < ways; ++w) {
-                const int i = w * lanes * at_once + rest;
-                const float f = tops[i] == kNegInf ? 0.0f : exp2_hw(tops[i] - all);
-                l = __builtin_fmaf(totals[i], f, l);
+            const float t4 = fmaxf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), top);
+            const float ref = t4 == kNegInf ? 0.0f : t4, f = exp2_hw(top - ref);
+            l *= f;
 #pragma unroll
-                for (int y = 0; y < 4; ++y) sum[y] = __builtin_fmaf(sums[i][y], f, sum[y]);
+            for (int y = 0; y < 4; ++y) sum[y] *= f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float w = exp2_hw(m4[k] - ref);
+                l = __builtin_fmaf(l4[k], w, l);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) sum[y] = __builtin_fmaf(s4[k][y], w, sum[y]);
             }
-            const float f = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] = l == 0.0f ? 0.0f : sum[i] * f;
-            const size_t row = (size_t)seq * (size_t)a.nq + (size_t)(h * a.group + first + c);
-            store4_from_f32(a.out, a.dtype, row * (size_t)a.head_dim + x, sum);
+            top = t4;
         }
-        c0 += at_once;
     }
+    sums[tid] = sum;
+    totals[tid] = l;
+    tops[tid] = top;
+    __syncthreads();
+    if (way != 0) return;
+    for (uint32_t w = 0; w < ways; ++w) top = fmaxf(top, tops[w * lanes + tid]);
+    l = 0.0f;
+    sum = f32x4{0, 0, 0, 0};
+    for (uint32_t w = 0; w < ways; ++w) {
+        const uint32_t i = w * lanes + tid;
+        const float f = tops[i] == kNegInf ? 0.0f : exp2_hw(tops[i] - top);
+        l = __builtin_fmaf(totals[i], f, l);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) sum[y] = __builtin_fmaf(sums[i][y], f, sum[y]);
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = l == 0.0f ? 0.0f : sum[i] * f;
+    store4_from_f32(a.out, a.dtype, (size_t)q_row * (size_t)a.head_dim + x, sum);
 }
 
 // The kernel of a cache type, the narrowest that holds head_dim.

@@ -87,7 +87,7 @@ int launch_prompt(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipS
 // Shares of a call's single tokens: as many blocks as the GPU holds at once, or the most units there can be.
 struct SplitPlan {
     int tiles, cols, shares;
-    int64_t bytes;
+    int64_t ranges, bytes;  // of the part ranges, and of all
 };
 SplitPlan split_plan(int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages, int64_t page_size, int64_t head_dim) {
     SplitPlan p;
@@ -99,22 +99,23 @@ SplitPlan split_plan(int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages,
     p.tiles = (int)tiles;
     p.cols = (int)(group < 16 ? group : 16);
     p.shares = (int)shares;
-    p.bytes = 2 * shares * p.cols * (head_dim + 2) * 4;
+    p.ranges = (n_seqs * tiles * (int64_t)sizeof(PartRange) + 15) / 16 * 16;
+    p.bytes = p.ranges + 2 * shares * p.cols * (head_dim + 2) * 4;
     return p;
 }
 
 template <typename TC, bool HIGH>
-int launch_split(const AttnArgs& a, const SplitPlan& p, float* ws, hipStream_t s) {
+int launch_split(const AttnArgs& a, const SplitPlan& p, char* ws, hipStream_t s) {
     return with_tile_kernel<TC, HIGH>(a.head_dim, [&](auto k) {
         using K = decltype(k);
-        const SplitArgs sp{p.tiles, p.cols, p.shares, ws};
+        const SplitArgs sp{p.tiles, p.cols, p.shares, reinterpret_cast<PartRange*>(ws), reinterpret_cast<float*>(ws + p.ranges)};
         const int st = launch(paged_split_kernel<K>, dim3((unsigned)p.shares), kAttnThreads, s, a, sp);
         if (st != SPH_OK) return st;
-        return launch(paged_join_kernel<K::kStep>, dim3((unsigned)(a.pages.n_seqs * p.tiles)), kAttnThreads, s, a, sp);
+        return launch(paged_join_kernel, dim3((unsigned)a.n_rows * (unsigned)a.nq), kAttnThreads, s, a, sp);
     });
 }
 
-int dispatch_split(const AttnArgs& a, int cache_dtype, const SplitPlan& p, float* ws, hipStream_t s) {
+int dispatch_split(const AttnArgs& a, int cache_dtype, const SplitPlan& p, char* ws, hipStream_t s) {
     return with_float_type(cache_dtype, [&](auto tc) -> int {
         using TC = decltype(tc);
         if constexpr (!__is_same(TC, float)) {
@@ -141,9 +142,9 @@ extern "C" int sph_paged_attention(const void* q, void* out, int64_t n_q_heads, 
     if (st != SPH_OK) return st;
     if (n_seqs == 0) return SPH_OK;
     const SplitPlan p = split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim);
-    if (n_seqs * (int64_t)p.tiles * kAttnThreads > UINT32_MAX) return SPH_EINVAL;
+    if (n_seqs * n_q_heads * kAttnThreads > UINT32_MAX) return SPH_EINVAL;
     if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < p.bytes) return SPH_EINVAL;
-    return dispatch_split(a, cache_dtype, p, static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
+    return dispatch_split(a, cache_dtype, p, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
 }
 
 extern "C" int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype,

@@ -78,15 +78,26 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
 
     const TC *kc = static_cast<const TC*>(a.kc), *vc = static_cast<const TC*>(a.vc);
     const uint32_t head_rows = (uint32_t)t.h * a.pages.page.d;
-    auto row_at = [&](uint32_t t0) -> uint32_t {  // the pool row of key t0 + lane
+    // The table's entry for key t0 + lane, asked for two steps ahead, and the key's pool row.
+    auto entry_at = [&](uint32_t t0) { return a.pages.entry(t.seq, t0 + (uint32_t)lane < hi ? t0 + (uint32_t)lane : hi - 1); };
+    auto row_at = [&](uint32_t t0, uint32_t id) -> uint32_t {
         const uint32_t k = t0 + (uint32_t)lane;
-        if (k < lo || k >= hi) return kNoRow;
-        const uint32_t r = a.pages.row(t.seq, k);
-        if (r == kNoRow) {
-            if (a.bad != nullptr) *a.bad = 1;
-            return kNoRow;
+        const uint32_t r = a.pages.row_in(id, k < hi ? k : hi - 1);
+        if (k >= lo && k < hi && r == kNoRow && a.bad != nullptr) *a.bad = 1;
+        return k < hi && r != kNoRow ? r + head_rows : kNoRow;
+    };
+    auto is_key = [&](uint32_t t0, uint32_t rows) { return __ballot(rows != kNoRow && t0 + (uint32_t)lane >= lo); };
+    const bool by_16 = a.pages.page.d % 16 == 0;  // 16 neighbouring keys share a page
+    const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+    // The row of the step's key 16 block + i; rows of lanes in one block follow its first.
+    auto pool_row = [&](uint32_t rows, int block, int i) -> uint32_t {
+        uint32_t r;
+        if (by_16) {
+            r = __builtin_amdgcn_readlane(rows, 16 * block);
+            return (r == kNoRow ? 0u : r) + (uint32_t)i;
         }
-        return r + head_rows;
+        r = __shfl(rows, 16 * block + i);
+        return r == kNoRow ? 0u : r;
     };
     // This thread's part of a step's K and V, as it comes from memory. Row 0 stands in for a missing one: its scores
     // are masked, and as V it is cleared on the way to LDS, since 0 · inf is not 0.
@@ -97,20 +108,21 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int piece = i * kAttnThreads + tid, row = piece / CH, d = 8 * (piece % CH);
-            const uint32_t r = __shfl(rows, row);
+            const int block = (i * kAttnThreads + wave_u * kWave) / CH / 16;  // the wave's rows lie in one
+            const uint32_t r = pool_row(rows, block, row % 16);
             kr[i] = u32x4{0, 0, 0, 0};
-            if (EXACT || d < D) kr[i] = *reinterpret_cast<const u32x4*>(kc + (size_t)(r == kNoRow ? 0u : r) * (size_t)D + d);
+            if (EXACT || d < D) kr[i] = *reinterpret_cast<const u32x4*>(kc + (size_t)r * (size_t)D + d);
         }
 #pragma unroll
         for (int u = 0; u < VU; ++u)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t r = __shfl(rows, 4 * v_quad + e);
+                const uint32_t r = pool_row(rows, wave_u, 4 * (v_quad % 4) + e);
                 const int d = VE * (v_oct + 16 * u);
 #pragma unroll
                 for (int w = 0; w < VW; ++w) vr[u][e][w] = 0u;
                 if (EXACT || d < D) {
-                    const TC* p = vc + (size_t)(r == kNoRow ? 0u : r) * (size_t)D + d;
+                    const TC* p = vc + (size_t)r * (size_t)D + d;
                     if constexpr (VW == 4) {
                         const u32x4 x = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
@@ -165,18 +177,22 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
 
     uint32_t t0 = part.start;
     const uint32_t end = part.end;  // steps [start, end) of 64 keys
-    uint32_t rows = row_at(t0), rows_next = row_at(t0 + kPromptKeys);
+    uint32_t rows = kNoRow, id_next = 0;
     if (t0 < end) {
+        const uint32_t id = entry_at(t0);
+        id_next = entry_at(t0 + kPromptKeys);
+        rows = row_at(t0, id);
         load_step(rows);
-        store_step(0, __ballot(rows != kNoRow));
+        store_step(0, is_key(t0, rows));
     }
     __syncthreads();
     for (int buf = 0; t0 < end; t0 += kPromptKeys, buf ^= 1) {
         const bool more = t0 + kPromptKeys < end;
-        const uint32_t rows_after = row_at(t0 + 2 * kPromptKeys);
-        if (more) load_step(rows_next);
+        const uint32_t rows_next = row_at(t0 + kPromptKeys, id_next);
+        id_next = entry_at(t0 + 2 * kPromptKeys);
+        load_step(rows_next);  // (Past the end too: loads in a branch would all be waited for where any is.)
 
-        const uint64_t there = __ballot(rows != kNoRow);
+        const uint64_t there = is_key(t0, rows);
         const int last = (int)t0 + kPromptKeys - 1;
         const bool none = n_cols <= 0 || (pos_last < (int)t0 && prefix <= (int)t0) ||
                           (a.window > 0 && pos_first - last >= a.window);
@@ -253,9 +269,8 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
                     acc[d] = mma32<TC>(v, p[i], acc[d]);
                 }
         }
-        if (more) store_step(buf ^ 1, __ballot(rows_next != kNoRow));
+        if (more) store_step(buf ^ 1, is_key(t0 + kPromptKeys, rows_next));
         rows = rows_next;
-        rows_next = rows_after;
         __syncthreads();
     }
 

@@ -44,6 +44,14 @@ struct PagedTable {
         return id < (uint32_t)n_pages ? id * (uint32_t)n_kv * page.d + (t - p * page.d) : kNoRow;
     }
 
+    // The same in two parts, so that the entry can be asked for well ahead of its use: t < capacity, and no branch.
+    __device__ __forceinline__ uint32_t entry(int seq, uint32_t t) const {
+        return (uint32_t)table[(size_t)seq * (size_t)max_pages + page.quotient(t)];
+    }
+    __device__ __forceinline__ uint32_t row_in(uint32_t id, uint32_t t) const {
+        return id < (uint32_t)n_pages ? id * (uint32_t)n_kv * page.d + (t - page.quotient(t) * page.d) : kNoRow;
+    }
+
     // Keys of sequence b that the table can name: its length, cut at the capacity (and then flagged, by one lane).
     __device__ __forceinline__ int keys(int b, int32_t* bad, bool tell) const {
         const int len = lens[b];
