@@ -41,6 +41,12 @@ struct AttnArgs {
     float scale, cap;
 };
 
+// Parts that a chunk's keys are taken in, and where they go.
+struct ChunkSplit {
+    int splits;
+    float* part;  // [splits][n_rows · nq][head_dim] sums, then [splits][n_rows · nq][2] m and l
+};
+
 namespace {
 
 constexpr int kWave = 64;
@@ -505,10 +511,6 @@ struct TileKernel {
 // A chunk call's blocks take (sequence, tile of rows, kv head), and, where these are fewer than the GPU holds, equal
 // parts of the tile's keys, which paged_chunk_join_kernel sums. Which sequences the tiles belong to follows from cu_q
 // on the device: the grid has the most tiles there can be.
-struct ChunkSplit {
-    int splits;
-    float* part;  // [splits][n_rows · nq][head_dim] sums, then [splits][n_rows · nq][2] m and l
-};
 struct ChunkPart {
     int split;
     uint32_t lo, hi;      // the keys
@@ -653,7 +655,7 @@ struct SplitRange {
     uint32_t lo, hi, start, steps;
     __device__ __forceinline__ SplitRange(const AttnArgs& a, int b) {
         len = a.pages.lens[b];
-        hi = (uint32_t)a.pages.keys(b, nullptr, false);
+        hi = len < 0 ? 0u : (uint32_t)(len < a.pages.capacity ? len : a.pages.capacity);
         lo = a.window > 0 && len > a.window ? (uint32_t)(len - a.window) : 0u;
         if (lo > hi) lo = hi;
         start = lo & ~31u;
@@ -662,11 +664,17 @@ struct SplitRange {
     }
 };
 
-// `shares` of `total` units, none of them empty.
+// `shares` of `total` units, none of them empty. A double's quotient, cut, is the integers': their own distance from the
+// next integer, at least 1 / divisor, is more than its rounding while units stay below 2^43. (Integer divisions of 64
+// bits are some hundred operations each, in a row at every block's start.)
 __device__ __forceinline__ int64_t share_count(int64_t total, int shares) { return total < shares ? total : shares; }
-__device__ __forceinline__ int64_t share_start(int64_t share, int64_t total, int64_t shares) { return share * total / shares; }
+__device__ __forceinline__ int64_t share_start(int64_t share, int64_t total, int64_t shares) {
+    return (int64_t)((double)(share * total) / (double)shares);
+}
 // The share that unit u is in: the largest with share_start <= u.
-__device__ __forceinline__ int64_t share_of(int64_t u, int64_t total, int64_t shares) { return ((u + 1) * shares - 1) / total; }
+__device__ __forceinline__ int64_t share_of(int64_t u, int64_t total, int64_t shares) {
+    return (int64_t)((double)((u + 1) * shares - 1) / (double)total);
+}
 
 template <typename K>
 __global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_split_kernel(AttnArgs a, SplitArgs sp) {
@@ -681,9 +689,9 @@ __global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_split_ker
     const int tiles_per_head = sp.tiles_per_seq / a.pages.n_kv;
     for (int64_t u = begin; u < end; ++seq, within = 0) {
         const SplitRange<K::kStep> r(a, seq);
-        a.pages.keys(seq, a.bad, threadIdx.x == 0);
+        if (r.len > a.pages.capacity && a.bad != nullptr && threadIdx.x == 0) *a.bad = 1;
         for (; u < end && within < (int64_t)r.steps * sp.tiles_per_seq;) {
-            const int tile = (int)(within / r.steps);
+            const int tile = (int)((double)within / (double)r.steps);
             const uint32_t step = (uint32_t)(within - (int64_t)tile * r.steps);
             uint32_t n = r.steps - step;
             if ((int64_t)n > end - u) n = (uint32_t)(end - u);
@@ -726,6 +734,30 @@ __global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_split_ker
             within += n;
         }
     }
+}
+
+// One block per (sequence, tile), where the table holds too few keys for a split to gain what its second launch costs.
+template <typename K>
+__global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_whole_kernel(AttnArgs a, int tiles_per_seq) {
+    __shared__ typename K::Shared sm;
+    const int seq = blockIdx.x / tiles_per_seq, tile = blockIdx.x - seq * tiles_per_seq;
+    const int tiles_per_head = tiles_per_seq / a.pages.n_kv;
+    const SplitRange<K::kStep> r(a, seq);
+    if (r.len > a.pages.capacity && a.bad != nullptr && threadIdx.x == 0) *a.bad = 1;
+    Tile t;
+    t.seq = t.row0 = seq;
+    t.h = tile / tiles_per_head;
+    t.first = 16 * (tile - t.h * tiles_per_head);
+    t.rows = a.group;
+    t.pos0 = r.len - 1;
+    K k;
+    k.attend(a, sm, t, r.lo, r.hi, [&](int c, int d, float, float l, f32x4 sum) {
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = l == 0.0f ? 0.0f : sum[i] * f;
+        const size_t row = (size_t)seq * (size_t)a.nq + (size_t)(t.h * a.group + t.first + c);
+        store4_from_f32(a.out, a.dtype, row * (size_t)a.head_dim + d, sum);
+    });
 }
 
 // One block per (sequence, query head): nothing where one share held its tile, else the sum of its parts, 4 channels a
@@ -808,6 +840,10 @@ int with_tile_kernel(int head_dim, F&& f) {
 }
 
 }  // namespace
+
+// Chunks of one half type (attention_prompt.hip).
+constexpr int kPromptRows = 128;
+int launch_prompt(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) __attribute__((visibility("hidden")));
 
 // The checks of both entry points; fills `a`.
 int attn_args(AttnArgs& a, const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype, const int32_t* cu_q,

@@ -1,5 +1,5 @@
 // attention.hip — entry points of attention over the paged KV cache (kernels and their mathematics: attention.h).
-#include "attention_prompt.h"
+#include "attention.h"
 
 #include <math.h>
 
@@ -70,37 +70,29 @@ int launch_tiles(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipSt
         return launch(paged_tiles_kernel<decltype(k)>, dim3(blocks), kAttnThreads, s, a, sp);
     });
 }
-template <typename TC>
-int launch_prompt(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) {
-    auto go = [&](auto kernel) { return launch(kernel, dim3(blocks), kAttnThreads, s, a, sp); };
-    switch (a.head_dim) {
-    case 64: return go(paged_prompt_kernel<TC, 64, true>);
-    case 128: return go(paged_prompt_kernel<TC, 128, true>);
-    case 256: return go(paged_prompt_kernel<TC, 256, true>);
-    default:
-        return a.head_dim < 64    ? go(paged_prompt_kernel<TC, 64, false>)
-               : a.head_dim < 128 ? go(paged_prompt_kernel<TC, 128, false>)
-                                  : go(paged_prompt_kernel<TC, 256, false>);
-    }
-}
-
-// Shares of a call's single tokens: as many blocks as the GPU holds at once, or the most units there can be.
+// Shares of a call's single tokens: as many blocks as the GPU holds at once, or the most units there can be. Where no
+// sequence can have more than 512 keys, four block steps of most types (by its table or the window), a block takes a
+// sequence's tile whole, in one launch (one sequence of 333 keys 7.4 us; split 11.2).
 struct SplitPlan {
+    bool whole;
     int tiles, cols, shares;
     int64_t ranges, bytes;  // of the part ranges, and of all
 };
-SplitPlan split_plan(int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages, int64_t page_size, int64_t head_dim) {
+SplitPlan split_plan(int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages, int64_t page_size, int64_t head_dim,
+                     int64_t window) {
     SplitPlan p;
+    const int64_t capacity = max_pages * page_size;
+    p.whole = capacity <= 512 || (window > 0 && window <= 512);
     const int64_t group = nq / nkv;
     const int64_t tiles = (group + 15) / 16 * nkv;
-    const int64_t steps = max_pages * page_size / 64 + 1;  // the smaller of the kernels' steps
+    const int64_t steps = capacity / 64 + 1;  // the smaller of the kernels' steps
     int64_t shares = 256 * (head_dim > 128 ? 1 : 2);
     if ((__int128)n_seqs * tiles * steps < shares) shares = n_seqs * tiles * steps;
     p.tiles = (int)tiles;
     p.cols = (int)(group < 16 ? group : 16);
     p.shares = (int)shares;
     p.ranges = (n_seqs * tiles * (int64_t)sizeof(PartRange) + 15) / 16 * 16;
-    p.bytes = p.ranges + 2 * shares * p.cols * (head_dim + 2) * 4;
+    p.bytes = p.whole ? 0 : p.ranges + 2 * shares * p.cols * (head_dim + 2) * 4;
     return p;
 }
 
@@ -108,6 +100,7 @@ template <typename TC, bool HIGH>
 int launch_split(const AttnArgs& a, const SplitPlan& p, char* ws, hipStream_t s) {
     return with_tile_kernel<TC, HIGH>(a.head_dim, [&](auto k) {
         using K = decltype(k);
+        if (p.whole) return launch(paged_whole_kernel<K>, dim3((unsigned)(a.pages.n_seqs * p.tiles)), kAttnThreads, s, a, p.tiles);
         const SplitArgs sp{p.tiles, p.cols, p.shares, reinterpret_cast<PartRange*>(ws), reinterpret_cast<float*>(ws + p.ranges)};
         const int st = launch(paged_split_kernel<K>, dim3((unsigned)p.shares), kAttnThreads, s, a, sp);
         if (st != SPH_OK) return st;
@@ -141,9 +134,9 @@ extern "C" int sph_paged_attention(const void* q, void* out, int64_t n_q_heads, 
                              nullptr, bad_page_flag);
     if (st != SPH_OK) return st;
     if (n_seqs == 0) return SPH_OK;
-    const SplitPlan p = split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim);
+    const SplitPlan p = split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, a.window);
     if (n_seqs * n_q_heads * kAttnThreads > UINT32_MAX) return SPH_EINVAL;
-    if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < p.bytes) return SPH_EINVAL;
+    if (p.bytes > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < p.bytes)) return SPH_EINVAL;
     return dispatch_split(a, cache_dtype, p, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
 }
 
@@ -175,7 +168,7 @@ extern "C" int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_h
     const unsigned n = (unsigned)blocks;
     int r;
     if (prompt) {
-        r = dtype == SPH_F16 ? launch_prompt<f16>(a, n, sp, s) : launch_prompt<bf16>(a, n, sp, s);
+        r = launch_prompt(a, n, sp, s);
     } else {
         r = with_float_type(cache_dtype, [&](auto tc) { return launch_tiles<decltype(tc), true>(a, n, sp, s); });
     }
@@ -189,7 +182,7 @@ extern "C" int64_t sph_paged_attention_workspace(int64_t n_q_heads, int64_t n_kv
     if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads != 0 || n_seqs < 0 || max_pages < 0 || page_size < 1 ||
         head_dim < 1 || head_dim > 256)
         return SPH_EINVAL;
-    return sph::split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim).bytes;
+    return sph::split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, 0).bytes;
 }
 
 extern "C" int64_t sph_paged_attention_chunk_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs,

@@ -1,4 +1,4 @@
-// attention_prompt.h — the kernel of chunks whose q and cache are one half type: 128 rows a block (mathematics and
+// attention_prompt.hip — the kernel of chunks whose q and cache are one half type: 128 rows a block (mathematics and
 // the argument block: attention.h).
 //
 // Four waves of 32 columns (rows of q: tokens and the query heads of one kv head, so that a block reads its keys once
@@ -13,14 +13,12 @@
 //    4 tokens by 8 channels with 16 v_perm_b32 on the way, once for the four waves.
 // Two buffers: the next step's rows are on their way into registers while this step is computed, and are written to
 // the other buffer after it; one barrier a step.
-#pragma once
-
 #include "attention.h"
 
 namespace sph {
 namespace {
 
-constexpr int kPromptRows = 128, kPromptKeys = 64;
+constexpr int kPromptKeys = 64;
 
 template <typename TC>
 __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -300,5 +298,24 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
     }
 }
 
+template <typename TC>
+int launch_prompt_of(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) {
+    auto go = [&](auto kernel) { return launch(kernel, dim3(blocks), kAttnThreads, s, a, sp); };
+    switch (a.head_dim) {
+    case 64: return go(paged_prompt_kernel<TC, 64, true>);
+    case 128: return go(paged_prompt_kernel<TC, 128, true>);
+    case 256: return go(paged_prompt_kernel<TC, 256, true>);
+    default:
+        return a.head_dim < 64    ? go(paged_prompt_kernel<TC, 64, false>)
+               : a.head_dim < 128 ? go(paged_prompt_kernel<TC, 128, false>)
+                                  : go(paged_prompt_kernel<TC, 256, false>);
+    }
+}
+
 }  // namespace
+
+int launch_prompt(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) {
+    return a.dtype == SPH_F16 ? launch_prompt_of<f16>(a, blocks, sp, s) : launch_prompt_of<bf16>(a, blocks, sp, s);
+}
+
 }  // namespace sph
