@@ -5,14 +5,11 @@
 // for the whole group) share steps of 64 keys through LDS, on 32x32x16 matrix instructions. Scores are transposed
 // (S^T = K Q^T) as in the 16-column kernel: lane (j = lane % 32, h = lane / 32) holds column j's scores of tokens 8b +
 // 4h + 0..3, which is the order in which it feeds them back as the second operand, so weights never leave their lane.
-// In LDS
-//  - K lies as it comes, rows of DP channels in 16-byte pieces, piece c of row r at c ^ (r & 7): the 8 rows that a
-//    quarter of a read touches are in 8 different groups of banks;
-//  - V lies transposed, 64 tokens a channel, 8 pieces of 8 tokens in the order of the weights' slots (tokens 16m +
-//    4h + 0..3 and 16m + 8 + 4h + 0..3 are piece 2m + h), piece c of channel d at c ^ ((d ^ d >> 3) & 7). A thread turns
-//    4 tokens by 8 channels with 16 v_perm_b32 on the way, once for the four waves.
-// Two buffers: the next step's rows are on their way into registers while this step is computed, and are written to
-// the other buffer after it; one barrier a step.
+// Both lie in LDS as they come, rows of DP channels in 16-byte pieces, piece c of row r at c ^ (r & 7), so that what a
+// read touches at once (8 rows of K, 8 rows of V by 64 bytes) lies in different banks. They go there straight from
+// memory (16 bytes a lane; a wave's lanes fill 1 KB in a row, so the swap is in which piece a lane asks for), into the
+// other of two buffers while a step is computed: no registers hold them, no instruction moves them. V is read
+// transposed (ds_read_b64_tr_b16: of 4 rows by 16 channels, a channel's 4 values to a lane). One barrier a step.
 #include "attention.h"
 
 namespace sph {
@@ -26,6 +23,15 @@ __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+// 16 bytes a lane from `from` to LDS at `to` (the wave's, its lanes in a row).
+__device__ __forceinline__ void to_lds(const void* from, void* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to,
+                                     16, 0, 0);
 }
 
 template <typename TC, int DP>
@@ -42,10 +48,7 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
     constexpr int KS = DP / 16;                    // k steps of a score
     constexpr int DB = DP / 32;                    // blocks of channels
     constexpr int CH = DP / 8;                     // 16-byte pieces of a row
-    constexpr int KL = kPromptKeys * CH / kAttnThreads;  // pieces of K per thread and step
-    constexpr int VE = DP == 64 ? 4 : 8;           // channels of V that a thread turns
-    constexpr int VU = 16 * (DP / VE) / kAttnThreads;
-    constexpr int VW = VE / 2;
+    constexpr int PL = kPromptKeys * CH / kAttnThreads;  // pieces of K, and of V, per thread and step
     constexpr float kLift = __is_same(TC, f16) ? 7.0f : 0.0f;
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, j = lane % 32, h = lane / 32;
     const int D = EXACT ? DP : a.head_dim;
@@ -97,69 +100,49 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
         r = __shfl(rows, 16 * block + i);
         return r == kNoRow ? 0u : r;
     };
-    // This thread's part of a step's K and V, as it comes from memory. Row 0 stands in for a missing one: its scores
-    // are masked, and as V it is cleared on the way to LDS, since 0 · inf is not 0.
-    u32x4 kr[KL];
-    uint32_t vr[VU][4][VW];
-    const int v_oct = (tid & 7) | ((tid >> 4) & 1) << 3, v_quad = ((tid >> 3) & 1) << 1 | ((tid >> 5) & 1) | (tid >> 6) << 2;
-    auto load_step = [&](uint32_t rows) {
+    // A step's rows of K and V on their way to LDS. Row 0 stands in for a missing one: its scores are masked, and as V it
+    // is cleared when it has arrived, since 0 · inf is not 0. Channels past D are not asked for; they are zeros from
+    // the start.
+    auto load_step = [&](uint32_t rows, int buf) {
 #pragma unroll
-        for (int i = 0; i < KL; ++i) {
-            const int piece = i * kAttnThreads + tid, row = piece / CH, d = 8 * (piece % CH);
+        for (int i = 0; i < PL; ++i) {
+            const int piece = i * kAttnThreads + tid, row = piece / CH, d = 8 * ((piece % CH) ^ (row & 7));
             const int block = (i * kAttnThreads + wave_u * kWave) / CH / 16;  // the wave's rows lie in one
-            const uint32_t r = pool_row(rows, block, row % 16);
-            kr[i] = u32x4{0, 0, 0, 0};
-            if (EXACT || d < D) kr[i] = *reinterpret_cast<const u32x4*>(kc + (size_t)r * (size_t)D + d);
-        }
-#pragma unroll
-        for (int u = 0; u < VU; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t r = pool_row(rows, wave_u, 4 * (v_quad % 4) + e);
-                const int d = VE * (v_oct + 16 * u);
-#pragma unroll
-                for (int w = 0; w < VW; ++w) vr[u][e][w] = 0u;
-                if (EXACT || d < D) {
-                    const TC* p = vc + (size_t)r * (size_t)D + d;
-                    if constexpr (VW == 4) {
-                        const u32x4 x = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) vr[u][e][w] = x[w];
-                    } else {
-                        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-                        vr[u][e][0] = x[0];
-                        vr[u][e][1] = x[1];
-                    }
-                }
+            const size_t at = (size_t)pool_row(rows, block, row % 16) * (size_t)D + d;
+            const int to = 8 * (i * kAttnThreads + wave_u * kWave);
+            if (EXACT || d < D) {
+                to_lds(kc + at, &sm.k[buf][to]);
+                to_lds(vc + at, &sm.v[buf][to]);
             }
+        }
     };
-    auto store_step = [&](int buf, uint64_t there) {
-        if (there != ~uint64_t(0)) {
+    auto arrive = [&](uint64_t there, int buf) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (there == ~uint64_t(0)) return;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (!((there >> (4 * v_quad + e)) & 1)) {
-#pragma unroll
-                    for (int u = 0; u < VU; ++u)
-#pragma unroll
-                        for (int w = 0; w < VW; ++w) vr[u][e][w] = 0u;
-                }
+        for (int i = 0; i < PL; ++i) {
+            const int piece = i * kAttnThreads + tid;
+            if (!((there >> (piece / CH)) & 1)) *reinterpret_cast<u32x4*>(&sm.v[buf][8 * piece]) = u32x4{0, 0, 0, 0};
         }
-#pragma unroll
-        for (int i = 0; i < KL; ++i) {
-            const int piece = i * kAttnThreads + tid, row = piece / CH, c = piece % CH;
-            *reinterpret_cast<u32x4*>(&sm.k[buf][row * DP + 8 * (c ^ (row & 7))]) = kr[i];
+    };
+    if constexpr (!EXACT) {
+        for (int i = tid; i < 2 * kPromptKeys * CH; i += kAttnThreads) {
+            reinterpret_cast<u32x4*>(sm.k)[i] = u32x4{0, 0, 0, 0};
+            reinterpret_cast<u32x4*>(sm.v)[i] = u32x4{0, 0, 0, 0};
         }
+        __syncthreads();
+    }
+    const int v_r7 = 4 * h + lane % 16 / 4, v_chunk = 2 * (lane / 16 % 2) + lane % 4 / 2;
+    auto read_v = [&](int buf, int d, int i) {  // channels 32 d + j, slots of keys 16 i
+        u32x4 x;
 #pragma unroll
-        for (int u = 0; u < VU; ++u)
-#pragma unroll
-            for (int n = 0; n < VE; ++n) {
-                const int d = VE * (v_oct + 16 * u) + n;
-                const uint32_t sel = n % 2 ? 0x07060302u : 0x05040100u;
-                const u32x2 x = {__builtin_amdgcn_perm(vr[u][1][n / 2], vr[u][0][n / 2], sel),
-                                 __builtin_amdgcn_perm(vr[u][3][n / 2], vr[u][2][n / 2], sel)};
-                const int piece = 2 * (v_quad / 4) + (v_quad & 1), half = (v_quad >> 1) & 1;
-                *reinterpret_cast<u32x2*>(&sm.v[buf][d * kPromptKeys + 8 * (piece ^ ((d ^ d >> 3) & 7)) + 4 * half]) = x;
-            }
+        for (int e = 0; e < 2; ++e) {
+            const uint16_t* p = &sm.v[buf][(16 * i + 8 * e + v_r7) * DP + 8 * ((4 * d + v_chunk) ^ v_r7) + 4 * (lane % 2)];
+            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p));
+            x[2 * e] = w[0];
+            x[2 * e + 1] = w[1];
+        }
+        return x;
     };
 
     float m = kNegInf, l = 0.0f;
@@ -180,15 +163,15 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
         const uint32_t id = entry_at(t0);
         id_next = entry_at(t0 + kPromptKeys);
         rows = row_at(t0, id);
-        load_step(rows);
-        store_step(0, is_key(t0, rows));
+        load_step(rows, 0);
+        arrive(is_key(t0, rows), 0);
     }
     __syncthreads();
     for (int buf = 0; t0 < end; t0 += kPromptKeys, buf ^= 1) {
         const bool more = t0 + kPromptKeys < end;
         const uint32_t rows_next = row_at(t0 + kPromptKeys, id_next);
         id_next = entry_at(t0 + 2 * kPromptKeys);
-        load_step(rows_next);  // (Past the end too: loads in a branch would all be waited for where any is.)
+        if (more) load_step(rows_next, buf ^ 1);
 
         const uint64_t there = is_key(t0, rows);
         const int last = (int)t0 + kPromptKeys - 1;
@@ -260,14 +243,9 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const int ch = 32 * d + j;
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(
-                        &sm.v[buf][ch * kPromptKeys + 8 * ((2 * i + h) ^ ((ch ^ ch >> 3) & 7))]);
-                    acc[d] = mma32<TC>(v, p[i], acc[d]);
-                }
+                for (int d = 0; d < DB; ++d) acc[d] = mma32<TC>(read_v(buf, d, i), p[i], acc[d]);
         }
-        if (more) store_step(buf ^ 1, is_key(t0 + kPromptKeys, rows_next));
+        if (more) arrive(is_key(t0 + kPromptKeys, rows_next), buf ^ 1);
         rows = rows_next;
         __syncthreads();
     }
