@@ -34,6 +34,20 @@ __device__ __forceinline__ void to_lds(const void* from, void* to) {
                                      16, 0, 0);
 }
 
+// The order of the N products just written and the reads (READS for each) that feed them: the reads run six products ahead.
+// Left alone, the scheduler reads for one product at a time and waits out LDS's latency before each.
+template <int N, int READS>
+__device__ __forceinline__ void ahead_of_products() {
+    constexpr int kAhead = 6, kMatrix = 0x008, kRead = 0x100;
+    __builtin_amdgcn_sched_group_barrier(kRead, kAhead * READS, 0);
+#pragma unroll
+    for (int i = 0; i < N - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMatrix, kAhead, 0);
+}
+
 template <typename TC, int DP>
 struct PromptShared {
     alignas(16) uint16_t k[2][kPromptKeys * DP];
@@ -192,6 +206,7 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
                     const u32x4 k = *reinterpret_cast<const u32x4*>(&sm.k[buf][row * DP + 8 * ((2 * c + h) ^ (row & 7))]);
                     s[b] = mma32<TC>(k, q[c], s[b]);
                 }
+            ahead_of_products<2 * KS, 1>();
             const bool seen = there == ~uint64_t(0) && pos_first >= 0 && (last <= pos_first || last < prefix) &&
                               (a.window == 0 || pos_last - (int)t0 < a.window);
             if (!plain) {
@@ -244,6 +259,7 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int d = 0; d < DB; ++d) acc[d] = mma32<TC>(read_v(buf, d, i), p[i], acc[d]);
+            ahead_of_products<4 * DB, 2>();
         }
         if (more) arrive(is_key(t0 + kPromptKeys, rows_next), buf ^ 1);
         rows = rows_next;
