@@ -5,8 +5,9 @@
 // for the whole group) share steps of 64 keys through LDS, on 32x32x16 matrix instructions. Scores are transposed
 // (S^T = K Q^T) as in the 16-column kernel: lane (j = lane % 32, h = lane / 32) holds column j's scores of tokens 8b +
 // 4h + 0..3, which is the order in which it feeds them back as the second operand, so weights never leave their lane.
-// Both lie in LDS as they come, rows of DP channels in 16-byte pieces, piece c of row r at c ^ (r & 7), so that what a
-// read touches at once (8 rows of K, 8 rows of V by 64 bytes) lies in different banks. They go there straight from
+// Both lie in LDS as they come, rows of DP channels in 16-byte pieces, piece c of row r at c ^ swap(r), so that what a
+// read touches at once (a piece of 8 and of 16 neighbouring rows of K; of V, 32 bytes of 4 neighbouring rows, and 64) lies
+// in different banks. They go there straight from
 // memory (16 bytes a lane; a wave's lanes fill 1 KB in a row, so the swap is in which piece a lane asks for), into the
 // other of two buffers while a step is computed: no registers hold them, no instruction moves them. V is read
 // transposed (ds_read_b64_tr_b16: of 4 rows by 16 channels, a channel's 4 values to a lane). One barrier a step.
@@ -47,6 +48,11 @@ __device__ __forceinline__ void ahead_of_products() {
     }
     __builtin_amdgcn_sched_group_barrier(kMatrix, kAhead, 0);
 }
+
+template <int CH>
+__device__ __forceinline__ constexpr int swap_k(int row) { return CH == 8 ? (row ^ (row >> 3 & 1)) & 7 : row & 15; }
+template <int CH>
+__device__ __forceinline__ constexpr int swap_v(int row) { return CH == 8 ? 2 * (row & 3) : 2 * (row & 3) ^ 8 * (row & 1); }
 
 template <typename TC, int DP>
 struct PromptShared {
@@ -120,14 +126,13 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
     auto load_step = [&](uint32_t rows, int buf) {
 #pragma unroll
         for (int i = 0; i < PL; ++i) {
-            const int piece = i * kAttnThreads + tid, row = piece / CH, d = 8 * ((piece % CH) ^ (row & 7));
+            const int piece = i * kAttnThreads + tid, row = piece / CH, c = piece % CH;
+            const int dk = 8 * (c ^ swap_k<CH>(row)), dv = 8 * (c ^ swap_v<CH>(row));
             const int block = (i * kAttnThreads + wave_u * kWave) / CH / 16;  // the wave's rows lie in one
-            const size_t at = (size_t)pool_row(rows, block, row % 16) * (size_t)D + d;
+            const size_t at = (size_t)pool_row(rows, block, row % 16) * (size_t)D;
             const int to = 8 * (i * kAttnThreads + wave_u * kWave);
-            if (EXACT || d < D) {
-                to_lds(kc + at, &sm.k[buf][to]);
-                to_lds(vc + at, &sm.v[buf][to]);
-            }
+            if (EXACT || dk < D) to_lds(kc + at + dk, &sm.k[buf][to]);
+            if (EXACT || dv < D) to_lds(vc + at + dv, &sm.v[buf][to]);
         }
     };
     auto arrive = [&](uint64_t there, int buf) {
@@ -146,12 +151,12 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
         }
         __syncthreads();
     }
-    const int v_r7 = 4 * h + lane % 16 / 4, v_chunk = 2 * (lane / 16 % 2) + lane % 4 / 2;
+    const int v_row = 4 * h + lane % 16 / 4, v_chunk = 2 * (lane / 16 % 2) + lane % 4 / 2;
     auto read_v = [&](int buf, int d, int i) {  // channels 32 d + j, slots of keys 16 i
         u32x4 x;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const uint16_t* p = &sm.v[buf][(16 * i + 8 * e + v_r7) * DP + 8 * ((4 * d + v_chunk) ^ v_r7) + 4 * (lane % 2)];
+            const uint16_t* p = &sm.v[buf][(16 * i + 8 * e + v_row) * DP + 8 * ((4 * d + v_chunk) ^ swap_v<CH>(v_row)) + 4 * (lane % 2)];
             const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p));
             x[2 * e] = w[0];
             x[2 * e + 1] = w[1];
@@ -203,7 +208,7 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const int row = 32 * b + j;
-                    const u32x4 k = *reinterpret_cast<const u32x4*>(&sm.k[buf][row * DP + 8 * ((2 * c + h) ^ (row & 7))]);
+                    const u32x4 k = *reinterpret_cast<const u32x4*>(&sm.k[buf][row * DP + 8 * ((2 * c + h) ^ swap_k<CH>(j))]);
                     s[b] = mma32<TC>(k, q[c], s[b]);
                 }
             ahead_of_products<2 * KS, 1>();
