@@ -389,9 +389,11 @@ int sph_rope_kv_append_paged(const void* q, void* q_out, int64_t n_q_heads, cons
  * dtype ∈ {F32, F16, BF16} for q and out; cache_dtype ∈ {F32, F16, BF16};
  * head_dim a multiple of 8, at most 256; q, out, kcache and vcache 16-byte
  * aligned; n_q_heads a multiple of n_kv_heads; scale finite. Sums and
- * softmax statistics are f32. workspace: device memory of
- * sph_paged_attention_workspace bytes, 16-byte aligned, whose contents need not be
- * kept between calls, of one stream at a time. `out` may be q. */
+ * softmax statistics are f32. workspace: device memory, 16-byte aligned, of one
+ * call at a time (calls of one stream may share it, and graphs replayed in one),
+ * whose contents do not matter before or after: with sph_paged_attention_workspace
+ * bytes or more the work is split over the keys as far as it pays, with fewer (0: NULL)
+ * less far. `out` may be q. */
 int sph_paged_attention(const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype,
                         const int32_t* seq_lens, const int32_t* block_table, int64_t n_seqs, int64_t max_pages,
                         int64_t head_dim, const void* kcache, const void* vcache, int cache_dtype, int64_t n_pages,
@@ -405,8 +407,8 @@ int sph_paged_attention(const void* q, void* out, int64_t n_q_heads, int64_t n_k
  * seq_lens[b]. The chunk's own keys are in the cache already
  * (sph_rope_kv_append_paged). Rows past cu_q[n_seqs] are left as they were.
  * Replaces the chunk form of WgpuContext::attention (as above; causal,
- * crates/sapient-models/src/forward/wgpu_engine.rs:575-607). workspace:
- * sph_paged_attention_chunk_workspace bytes. `out` must not overlap q. */
+ * crates/sapient-models/src/forward/wgpu_engine.rs:575-607). workspace: as
+ * above, sph_paged_attention_chunk_workspace bytes. `out` must not overlap q. */
 int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype,
                               const int32_t* cu_q, const int32_t* seq_lens, const int32_t* block_table, int64_t n_seqs,
                               int64_t max_pages, int64_t n_tokens, int64_t head_dim, const void* kcache,
@@ -414,8 +416,8 @@ int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_heads, int64
                               float softcap, int64_t window, const float* slopes, const int32_t* prefix_lens,
                               void* workspace, int64_t workspace_bytes, int32_t* bad_page_flag, void* stream);
 
-/* Host functions: the workspace of the two calls at these sizes, in bytes (0 or
- * more; negative: a status, for sizes the calls refuse). */
+/* Host functions: the most workspace that the two calls use at these sizes, in
+ * bytes (0 or more; negative: a status, for sizes the calls refuse). */
 int64_t sph_paged_attention_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_pages,
                                       int64_t page_size, int64_t head_dim);
 int64_t sph_paged_attention_chunk_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_pages,

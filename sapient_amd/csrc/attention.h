@@ -58,13 +58,38 @@ constexpr float kNegInf = -__builtin_inff();
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// tanh of a score: by its own exp where the output is half precision (absolute error about 2^-23, under a rounding of
-// the weights), the library's where it is f32.
+// What is done to a product q·k where it is more than a scale: the cap, and the slope's distance; the score in log2
+// units. The cap is cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1), its exp and reciprocal the hardware's where the
+// output is half precision (absolute error some 2^-23 of the cap, under a rounding of the weights), the library's tanh
+// where it is f32.
 template <bool ACCURATE>
-__device__ __forceinline__ float score_tanh(float x) {
-    if constexpr (ACCURATE) return tanhf(x);
-    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(exp2_hw(x * (2.0f * kLog2e)) + 1.0f);
-}
+struct ScoreForm {
+    float unit, grow, cap, slope;
+    // unit: what a product is multiplied by for a score in its own units
+    __device__ __forceinline__ ScoreForm(const AttnArgs& a, float unit_, int head) : unit(unit_ * kLog2e) {
+        cap = a.cap * kLog2e;
+        grow = a.cap == 0.0f ? 0.0f : ACCURATE ? unit_ / a.cap : 2.0f * kLog2e * unit_ / a.cap;
+        slope = a.slopes != nullptr ? a.slopes[head] * -kLog2e : 0.0f;
+    }
+    // s[i]: the products of keys at distances dist - at(i)
+    template <int N, typename At>
+    __device__ __forceinline__ void apply(const AttnArgs& a, float (&s)[N], float dist, At at) const {
+        if (a.cap != 0.0f) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if constexpr (ACCURATE) s[i] = cap * tanhf(s[i] * grow);
+                else s[i] = __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(exp2_hw(s[i] * grow) + 1.0f), cap);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] *= unit;
+        }
+        if (a.slopes != nullptr) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] = __builtin_fmaf(slope, fabsf(dist - (float)at(i)), s[i]);
+        }
+    }
+};
 
 template <typename TC>
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
@@ -84,11 +109,33 @@ __device__ __forceinline__ float widen_half(uint32_t w, int i) {
     return widen(TC{(uint16_t)(w >> (16 * i))});
 }
 
-// Element i of a float tensor of type dt.
-__device__ __forceinline__ float load_as_f32(const void* p, int dt, size_t i) {
-    if (dt == SPH_F32) return static_cast<const float*>(p)[i];
-    const uint16_t h = static_cast<const uint16_t*>(p)[i];
-    return dt == SPH_F16 ? widen(f16{h}) : widen(bf16{h});
+// f[s] = the E channels from d0 + s · step of a row of type dt (at element `at`), zeros from channel D on. One branch on the
+// type with all loads of it in flight together: asked for one by one, each in a branch of its own, they were waited for
+// one by one (16 us of a chunk's 19).
+template <int KS, int E>
+__device__ __forceinline__ void load_row_f32(const void* p, int dt, size_t at, int d0, int step, int D, float (&f)[KS][E]) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[s][e] = 0.0f;
+    if (dt == SPH_F32) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+            if (d0 + s * step < D) load_f32<float, E>(static_cast<const float*>(p) + at + d0 + s * step, f[s]);
+    } else {
+        uint32_t w[KS][E / 2];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) w[s][i] = 0u;
+            if (d0 + s * step < D) load_words<f16, E>(static_cast<const f16*>(p) + at + d0 + s * step, w[s]);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (dt == SPH_F16) words_to_f32<f16, E>(w[s], f[s]);
+            else words_to_f32<bf16, E>(w[s], f[s]);
+        }
+    }
 }
 __device__ __forceinline__ void store4_from_f32(void* p, int dt, size_t i, f32x4 v) {
     if (dt == SPH_F32) {
@@ -152,6 +199,35 @@ __device__ __forceinline__ uint64_t visible(uint64_t there, int t0, int pos, int
     return pos < 0 ? 0 : see & there;
 }
 
+// Pieces of the cache's type TC that q and the weights are written as, high one first. With one piece the weights'
+// rounding would add to an output of that type as much again as the output's own.
+template <typename TC, bool HIGH>
+struct Pieces {
+    // q: exact (f16 and bf16 into one another, f32 into bf16) or within 2^-22 (f32 into f16); weights for f32 outputs
+    static constexpr int q = !HIGH ? 1 : __is_same(TC, bf16) ? 3 : 2;
+    static constexpr int high = __is_same(TC, bf16) ? 3 : 2;
+};
+// The channels f of a row, of which the largest is `most`, as pieces of TC; brought to [1, 2) by a power of two before, so
+// that no piece leaves the type's range. Returns the power.
+template <typename TC, int NQ, int KS>
+__device__ __forceinline__ int split_row(const float (&f)[KS][8], float most, u32x4 (&q)[NQ][KS]) {
+    const int ex = most > 0.0f && most < __builtin_inff() ? ilogbf(most) : 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            float x = ldexpf(f[s][e], -ex), y = ldexpf(f[s][e + 1], -ex);
+#pragma unroll
+            for (int p = 0; p < NQ; ++p) {
+                const uint32_t w = narrow2<TC>(x, y);
+                q[p][s][e / 2] = w;
+                x -= widen_half<TC>(w, 0);
+                y -= widen_half<TC>(w, 1);
+            }
+        }
+    return ex;
+}
+
 // A tile's 16 columns: the rows (token i of the sequence's new ones, head h · group + c) with number i · group + c in
 // [first, first + 16) of `rows`, for kv head h.
 struct Tile {
@@ -172,11 +248,8 @@ struct TileKernel {
     static constexpr int KS = kF32 ? DP / 16 : DP / 32;    // 16-byte pieces of a K row per lane
     static constexpr int VT = ST / 4;                      // tokens of V per lane
     static constexpr int VW = E * (int)sizeof(TC) / 4;     // words of V per token and lane
-    // Pieces of the cache's type that q and the weights are written as, high one first. q: exact (f16 and bf16 into
-    // one another; f32 into bf16), or within 2^-22 (f32 into f16). Weights: with one piece their rounding would add
-    // to the output's as much again, so two; three where the output is f32 and a piece has 8 bits.
-    static constexpr int NQ = kF32 ? 1 : !HIGH ? 1 : __is_same(TC, bf16) ? 3 : 2;
-    static constexpr int NP = kF32 ? 1 : HIGH && __is_same(TC, bf16) ? 3 : 2;
+    static constexpr int NQ = kF32 ? 1 : Pieces<TC, HIGH>::q;
+    static constexpr int NP = kF32 ? 1 : HIGH ? Pieces<TC, HIGH>::high : 2;  // (two are free here: memory is waited for)
     // An f16 weight below 2^-14 loses bits: the reference is taken 2^7 lower, so that weights run up to 2^15.
     static constexpr float kLift = __is_same(TC, f16) ? 7.0f : 0.0f;
     static constexpr int kPasses = DP > 128 ? DP / 128 : 1;  // of the join over waves, 128 channels each
@@ -206,8 +279,6 @@ struct TileKernel {
         const int pos = t.pos0 + tok;
         const int pos_first = t.pos0 + t.first / a.group, pos_last = t.pos0 + (t.first + n_cols - 1) / a.group;
         const int prefix = a.prefix != nullptr ? a.prefix[t.seq] : 0;
-        const float slope = a.slopes != nullptr ? a.slopes[head] : 0.0f;
-        const float inv_cap = a.cap != 0.0f ? 1.0f / a.cap : 0.0f;
 
         // q, as the B operand: column j, channels of this lane's k slots.
         float unit = a.scale;
@@ -221,42 +292,25 @@ struct TileKernel {
                 if (EXACT || d < D) q[0][s] = *reinterpret_cast<const u32x4*>(static_cast<const TC*>(a.q) + q_at + d);
             }
         } else if constexpr (kF32) {
+            float f[KS][4];
+            load_row_f32(a.q, a.dtype, q_at, 4 * g, 16, D, f);
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = 16 * s + 4 * g + e;
-                    q[0][s][e] = __float_as_uint(EXACT || d < D ? load_as_f32(a.q, a.dtype, q_at + d) : 0.0f);
-                }
+                for (int e = 0; e < 4; ++e) q[0][s][e] = __float_as_uint(f[s][e]);
         } else {
-            // Brought to [1, 2) by a power of two, so that no piece leaves the type's range.
             float f[KS][8], most = 0.0f;
+            load_row_f32(a.q, a.dtype, q_at, 8 * g, 32, D, f);
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int d = 32 * s + 8 * g + e;
-                    f[s][e] = EXACT || d < D ? load_as_f32(a.q, a.dtype, q_at + d) : 0.0f;
-                    most = fmaxf(most, fabsf(f[s][e]));
-                }
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[s][e]));
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
-            const int ex = most > 0.0f && most < __builtin_inff() ? ilogbf(most) : 0;
-            unit = ldexpf(unit, ex);
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    float x = ldexpf(f[s][e], -ex), y = ldexpf(f[s][e + 1], -ex);
-#pragma unroll
-                    for (int p = 0; p < NQ; ++p) {
-                        const uint32_t w = narrow2<TC>(x, y);
-                        q[p][s][e / 2] = w;
-                        x -= widen_half<TC>(w, 0);
-                        y -= widen_half<TC>(w, 1);
-                    }
-                }
+            unit = ldexpf(unit, split_row<TC>(f, most, q));
         }
+
+        const ScoreForm<HIGH || kF32> form(a, unit, head);
 
         const TC *kc = static_cast<const TC*>(a.kc), *vc = static_cast<const TC*>(a.vc);
         const uint32_t head_rows = (uint32_t)t.h * a.pages.page.d;
@@ -370,22 +424,13 @@ struct TileKernel {
             const uint32_t last = t0 + ST - 1;
             const bool seen = whole && pos_first >= 0 && ((int)last <= pos_first || (int)last < prefix) &&
                               (a.window == 0 || pos_last - (int)t0 < a.window);
-            if (a.cap == 0.0f && a.slopes == nullptr) {
-                const float c = unit * kLog2e;
+            {
+                float x[4 * KB];
 #pragma unroll
-                for (int b = 0; b < KB; ++b)
+                for (int i = 0; i < 4 * KB; ++i) x[i] = s[i / 4][i % 4];
+                form.apply(a, x, (float)(pos - (int)t0 - 4 * g), [](int i) { return 16 * (i / 4) + i % 4; });
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[b][r] *= c;
-            } else {
-#pragma unroll
-                for (int b = 0; b < KB; ++b)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float x = s[b][r] * unit;
-                        if (a.cap != 0.0f) x = a.cap * score_tanh<HIGH || kF32>(x * inv_cap);
-                        if (a.slopes != nullptr) x -= slope * fabsf((float)(pos - (int)(t0 + 16 * b + 4 * g + r)));
-                        s[b][r] = x * kLog2e;
-                    }
+                for (int i = 0; i < 4 * KB; ++i) s[i / 4][i % 4] = x[i];
             }
             if (!seen) {
                 const uint32_t see = (uint32_t)visible(there, (int)t0, pos, prefix, a.window) >> (4 * g);
@@ -611,17 +656,36 @@ __global__ __launch_bounds__(kAttnThreads) void paged_chunk_join_kernel(AttnArgs
     const int64_t row = (int64_t)(q_row / (size_t)a.nq);
     if (row < a.pages.cu[0] || row >= a.pages.cu[a.pages.n_seqs]) return;
     const float* ml = sp.part + (size_t)sp.splits * all * (size_t)a.head_dim + 2 * q_row;
-    float top = kNegInf;
-    for (int s = 0; s < sp.splits; ++s) top = fmaxf(top, ml[2 * s * all]);
-    const float ref = top == kNegInf ? 0.0f : top;
-    float l = 0.0f;
+    float top = kNegInf, l = 0.0f;
     f32x4 sum = {0, 0, 0, 0};
-    for (int s = 0; s < sp.splits; ++s) {
-        const float f = exp2_hw(ml[2 * s * all] - ref);
-        const f32x4 p = *reinterpret_cast<const f32x4*>(sp.part + (s * all + q_row) * (size_t)a.head_dim + x);
-        l = __builtin_fmaf(ml[2 * s * all + 1], f, l);
+    // In groups of eight, whose loads are in flight together.
+    constexpr int kAhead = 8;
+    for (int s0 = 0; s0 < sp.splits; s0 += kAhead) {
+        float m_[kAhead], l_[kAhead];
+        f32x4 p_[kAhead];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sum[c] = __builtin_fmaf(p[c], f, sum[c]);
+        for (int k = 0; k < kAhead; ++k) {
+            const size_t s = s0 + k < sp.splits ? s0 + k : s0;
+            m_[k] = ml[2 * s * all];
+            l_[k] = ml[2 * s * all + 1];
+            p_[k] = *reinterpret_cast<const f32x4*>(sp.part + (s * all + q_row) * (size_t)a.head_dim + x);
+            if (s0 + k >= sp.splits) m_[k] = kNegInf;
+        }
+        float most = top;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) most = fmaxf(most, m_[k]);
+        const float ref = most == kNegInf ? 0.0f : most, f = exp2_hw(top - ref);
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] *= f;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const float w = exp2_hw(m_[k] - ref);
+            l = __builtin_fmaf(l_[k], w, l);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] = __builtin_fmaf(p_[k][c], w, sum[c]);
+        }
+        top = most;
     }
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -841,9 +905,9 @@ int with_tile_kernel(int head_dim, F&& f) {
 
 }  // namespace
 
-// Chunks of one half type (attention_prompt.hip).
+// Chunks over caches of a half type (attention_prompt.hip).
 constexpr int kPromptRows = 128;
-int launch_prompt(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) __attribute__((visibility("hidden")));
+int launch_prompt(const AttnArgs& a, int cache_dtype, unsigned blocks, const ChunkSplit& sp, hipStream_t s) __attribute__((visibility("hidden")));
 
 // The checks of both entry points; fills `a`.
 int attn_args(AttnArgs& a, const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype, const int32_t* cu_q,

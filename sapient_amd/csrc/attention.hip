@@ -14,7 +14,7 @@ int attn_args(AttnArgs& a, const void* q, void* out, int64_t n_q_heads, int64_t 
     if (!paged_ok(seq_lens, block_table, n_seqs, max_pages, n_pages, page_size, n_kv_heads, n_rows)) return SPH_EINVAL;
     if (n_q_heads < 1 || n_q_heads > INT32_MAX || n_q_heads % n_kv_heads != 0) return SPH_EINVAL;
     if (head_dim <= 0 || head_dim % 8 != 0 || head_dim > 256) return SPH_EINVAL;
-    if (n_rows * (n_q_heads / n_kv_heads) > INT32_MAX) return SPH_EINVAL;
+    if (n_rows * n_q_heads > INT32_MAX) return SPH_EINVAL;
     if (!isfinite(scale) || !isfinite(softcap) || softcap < 0.0f || window < 0) return SPH_EINVAL;
     if (!aligned(cu_q, 4) || !aligned(slopes, 4) || !aligned(prefix_lens, 4)) return SPH_EINVAL;
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(kcache, 16) || !aligned(vcache, 16)) return SPH_EINVAL;
@@ -40,37 +40,40 @@ int attn_args(AttnArgs& a, const void* q, void* out, int64_t n_q_heads, int64_t 
 
 namespace {
 
-// Parts of a chunk's keys, where its tiles alone are fewer than the blocks that the GPU holds: at most 16, of 512 keys or
-// more were the table full.
+// Parts of a chunk's keys, where its tiles alone are fewer than the blocks that the GPU holds: at most 16, of 256 keys or
+// more were the table full, and no more than fit the workspace. (Twice the blocks, for tiles of different lengths: nine
+// sequences of five tokens over up to 12000 keys 47 -> 58 us.)
 struct ChunkPlan {
     int64_t tiles;  // the most there can be, of one kv head: every sequence's end in at most one that is not full
     int splits;
     int64_t bytes;
 };
 ChunkPlan chunk_plan(int rows_per_tile, int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages, int64_t page_size,
-                     int64_t n_rows, int64_t head_dim) {
+                     int64_t n_rows, int64_t head_dim, int64_t workspace_bytes) {
     ChunkPlan p;
     p.tiles = n_rows * (nq / nkv) / rows_per_tile + (n_seqs < n_rows ? n_seqs : n_rows);
-    const int64_t blocks = p.tiles * nkv, slots = 256 * (head_dim > 128 ? 1 : 2), most = max_pages * page_size / 512;
+    const int64_t blocks = p.tiles * nkv, slots = 256 * (head_dim > 128 ? 1 : 2), most = max_pages * page_size / 256;
+    const int64_t part = n_rows * nq * (head_dim + 2) * 4;
     int64_t s = blocks > 0 ? slots / blocks : 1;
     if (s > 16) s = 16;
     if (s > most) s = most;
+    if (part > 0 && s > workspace_bytes / part) s = workspace_bytes / part;
     if (s < 1) s = 1;
     p.splits = (int)s;
-    p.bytes = s > 1 ? s * n_rows * nq * (head_dim + 2) * 4 : 0;
+    p.bytes = s > 1 ? s * part : 0;
     return p;
 }
 
-// Chunks of one half type take tiles of 128 rows, others of 16.
+// Chunks over caches of a half type take tiles of 128 rows, over f32 ones of 16.
 inline int chunk_rows(bool prompt) { return prompt ? kPromptRows : 16; }
 
-template <typename TC, bool HIGH>
 int launch_tiles(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) {
-    return with_tile_kernel<TC, HIGH>(a.head_dim, [&](auto k) {
+    return with_tile_kernel<float, true>(a.head_dim, [&](auto k) {
         return launch(paged_tiles_kernel<decltype(k)>, dim3(blocks), kAttnThreads, s, a, sp);
     });
 }
-// Shares of a call's single tokens: as many blocks as the GPU holds at once, or the most units there can be. Where no
+// Shares of a call's single tokens: as many blocks as the GPU holds at once, the most units there can be, or what fits the
+// workspace. Where no
 // sequence can have more than 512 keys, four block steps of most types (by its table or the window), a block takes a
 // sequence's tile whole, in one launch (one sequence of 333 keys 7.4 us; split 11.2).
 struct SplitPlan {
@@ -79,10 +82,9 @@ struct SplitPlan {
     int64_t ranges, bytes;  // of the part ranges, and of all
 };
 SplitPlan split_plan(int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages, int64_t page_size, int64_t head_dim,
-                     int64_t window) {
+                     int64_t window, int64_t workspace_bytes) {
     SplitPlan p;
     const int64_t capacity = max_pages * page_size;
-    p.whole = capacity <= 512 || (window > 0 && window <= 512);
     const int64_t group = nq / nkv;
     const int64_t tiles = (group + 15) / 16 * nkv;
     const int64_t steps = capacity / 64 + 1;  // the smaller of the kernels' steps
@@ -92,7 +94,10 @@ SplitPlan split_plan(int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages,
     p.cols = (int)(group < 16 ? group : 16);
     p.shares = (int)shares;
     p.ranges = (n_seqs * tiles * (int64_t)sizeof(PartRange) + 15) / 16 * 16;
-    p.bytes = p.whole ? 0 : p.ranges + 2 * shares * p.cols * (head_dim + 2) * 4;
+    const int64_t part = 2 * p.cols * (head_dim + 2) * 4;
+    if (p.shares > (workspace_bytes - p.ranges) / part) p.shares = (int)((workspace_bytes - p.ranges) / part);
+    p.whole = capacity <= 512 || (window > 0 && window <= 512) || workspace_bytes < p.ranges + 2 * part;
+    p.bytes = p.whole ? 0 : p.ranges + p.shares * part;
     return p;
 }
 
@@ -134,9 +139,10 @@ extern "C" int sph_paged_attention(const void* q, void* out, int64_t n_q_heads, 
                              nullptr, bad_page_flag);
     if (st != SPH_OK) return st;
     if (n_seqs == 0) return SPH_OK;
-    const SplitPlan p = split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, a.window);
     if (n_seqs * n_q_heads * kAttnThreads > UINT32_MAX) return SPH_EINVAL;
-    if (p.bytes > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < p.bytes)) return SPH_EINVAL;
+    const SplitPlan p = split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, a.window,
+                                   workspace == nullptr ? 0 : workspace_bytes);
+    if (!aligned(workspace, 16)) return SPH_EINVAL;
     return dispatch_split(a, cache_dtype, p, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
 }
 
@@ -158,9 +164,10 @@ extern "C" int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_h
     const uintptr_t bytes = (uintptr_t)n_q_heads * (uintptr_t)n_tokens * (uintptr_t)head_dim * dtype_size(dtype);
     const uintptr_t x = (uintptr_t)q, y = (uintptr_t)out;
     if (x < y + bytes && y < x + bytes) return SPH_EINVAL;  // a row's columns are read by one block and written by another
-    const bool prompt = dtype == cache_dtype && dtype != SPH_F32;
-    const ChunkPlan p = chunk_plan(chunk_rows(prompt), n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, n_tokens, head_dim);
-    if (p.bytes > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < p.bytes)) return SPH_EINVAL;
+    const bool prompt = cache_dtype != SPH_F32;
+    const ChunkPlan p = chunk_plan(chunk_rows(prompt), n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, n_tokens, head_dim,
+                                   workspace == nullptr ? 0 : workspace_bytes);
+    if (!aligned(workspace, 16)) return SPH_EINVAL;
     const __int128 blocks = (__int128)p.tiles * n_kv_heads * p.splits;
     if (blocks * kAttnThreads > UINT32_MAX) return SPH_EINVAL;
     const ChunkSplit sp{p.splits, static_cast<float*>(workspace)};
@@ -168,9 +175,9 @@ extern "C" int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_h
     const unsigned n = (unsigned)blocks;
     int r;
     if (prompt) {
-        r = launch_prompt(a, n, sp, s);
+        r = launch_prompt(a, cache_dtype, n, sp, s);
     } else {
-        r = with_float_type(cache_dtype, [&](auto tc) { return launch_tiles<decltype(tc), true>(a, n, sp, s); });
+        r = launch_tiles(a, n, sp, s);
     }
     if (r != SPH_OK || p.splits == 1) return r;
     const int64_t threads = n_tokens * n_q_heads * (head_dim / 4);
@@ -182,7 +189,7 @@ extern "C" int64_t sph_paged_attention_workspace(int64_t n_q_heads, int64_t n_kv
     if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads != 0 || n_seqs < 0 || max_pages < 0 || page_size < 1 ||
         head_dim < 1 || head_dim > 256)
         return SPH_EINVAL;
-    return sph::split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, 0).bytes;
+    return sph::split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, 0, INT64_MAX).bytes;
 }
 
 extern "C" int64_t sph_paged_attention_chunk_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs,
@@ -195,7 +202,7 @@ extern "C" int64_t sph_paged_attention_chunk_workspace(int64_t n_q_heads, int64_
     int64_t most = 0;
     for (const bool prompt : {false, true}) {
         const int64_t n = sph::chunk_plan(sph::chunk_rows(prompt), n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, n_tokens,
-                                          head_dim).bytes;
+                                          head_dim, INT64_MAX).bytes;
         if (n > most) most = n;
     }
     return most;

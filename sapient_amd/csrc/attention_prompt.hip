@@ -1,4 +1,4 @@
-// attention_prompt.hip — the kernel of chunks whose q and cache are one half type: 128 rows a block (mathematics and
+// attention_prompt.hip — the kernel of chunks over caches of a half type: 128 rows a block (mathematics and
 // the argument block: attention.h).
 //
 // Four waves of 32 columns (rows of q: tokens and the query heads of one kv head, so that a block reads its keys once
@@ -35,18 +35,18 @@ __device__ __forceinline__ void to_lds(const void* from, void* to) {
                                      16, 0, 0);
 }
 
-// The order of the N products just written and the reads (READS for each) that feed them: the reads run six products ahead.
-// Left alone, the scheduler reads for one product at a time and waits out LDS's latency before each.
-template <int N, int READS>
+// The order of the N operands just written, READS reads each, and their PRODUCTS products each: the reads run six operands
+// ahead. Left alone, the scheduler reads for one product at a time and waits out LDS's latency before each.
+template <int N, int READS, int PRODUCTS>
 __device__ __forceinline__ void ahead_of_products() {
     constexpr int kAhead = 6, kMatrix = 0x008, kRead = 0x100;
     __builtin_amdgcn_sched_group_barrier(kRead, kAhead * READS, 0);
 #pragma unroll
     for (int i = 0; i < N - kAhead; ++i) {
-        __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kMatrix, PRODUCTS, 0);
         __builtin_amdgcn_sched_group_barrier(kRead, READS, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(kMatrix, kAhead, 0);
+    __builtin_amdgcn_sched_group_barrier(kMatrix, kAhead * PRODUCTS, 0);
 }
 
 template <int CH>
@@ -61,14 +61,17 @@ struct PromptShared {
     Located located;
 };
 
-// EXACT: head_dim is DP.
-template <typename TC, int DP, bool EXACT>
-__global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_kernel(AttnArgs a, ChunkSplit sp) {
+// EXACT: head_dim is DP. HIGH: q is f32, or another half type than the cache; its pieces take the registers of a second
+// block a CU where rows are wider than 64.
+constexpr int prompt_blocks(int DP, bool HIGH) { return DP > 128 || (HIGH && DP > 64) ? 1 : 2; }
+template <typename TC, int DP, bool EXACT, bool HIGH>
+__global__ __launch_bounds__(kAttnThreads, prompt_blocks(DP, HIGH)) void paged_prompt_kernel(AttnArgs a, ChunkSplit sp) {
     __shared__ PromptShared<TC, DP> sm;
     constexpr int KS = DP / 16;                    // k steps of a score
     constexpr int DB = DP / 32;                    // blocks of channels
     constexpr int CH = DP / 8;                     // 16-byte pieces of a row
     constexpr int PL = kPromptKeys * CH / kAttnThreads;  // pieces of K, and of V, per thread and step
+    constexpr int NQ = Pieces<TC, HIGH>::q, NP = HIGH ? Pieces<TC, HIGH>::high : 1;
     constexpr float kLift = __is_same(TC, f16) ? 7.0f : 0.0f;
     const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, j = lane % 32, h = lane / 32;
     const int D = EXACT ? DP : a.head_dim;
@@ -86,16 +89,28 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
     const int pos_first = t.pos0 + wave_first / a.group;
     const int pos_last = t.pos0 + (wave_first + (n_cols > 0 ? n_cols : 1) - 1) / a.group;
     const int prefix = a.prefix != nullptr ? a.prefix[t.seq] : 0;
-    const float slope = a.slopes != nullptr ? a.slopes[head] : 0.0f;
     const size_t q_row = (size_t)(t.row0 + tok) * (size_t)a.nq + (size_t)head;
 
-    u32x4 q[KS];
+    u32x4 q[NQ][KS];
+    float scale = a.scale;
+    if constexpr (!HIGH) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        const int d = 16 * s + 8 * h;
-        q[s] = u32x4{0, 0, 0, 0};
-        if (EXACT || d < D) q[s] = *reinterpret_cast<const u32x4*>(static_cast<const TC*>(a.q) + q_row * (size_t)D + d);
+        for (int s = 0; s < KS; ++s) {
+            const int d = 16 * s + 8 * h;
+            q[0][s] = u32x4{0, 0, 0, 0};
+            if (EXACT || d < D) q[0][s] = *reinterpret_cast<const u32x4*>(static_cast<const TC*>(a.q) + q_row * (size_t)D + d);
+        }
+    } else {
+        float f[KS][8], most = 0.0f;
+        load_row_f32(a.q, a.dtype, q_row * (size_t)D, 8 * h, 16, D, f);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[s][e]));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        scale = ldexpf(scale, split_row<TC>(f, most, q));
     }
+    const ScoreForm<HIGH> form(a, scale, head);
 
     const TC *kc = static_cast<const TC*>(a.kc), *vc = static_cast<const TC*>(a.vc);
     const uint32_t head_rows = (uint32_t)t.h * a.pages.page.d;
@@ -172,8 +187,7 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
 
     const bool plain = a.cap == 0.0f && a.slopes == nullptr && a.scale > 0.0f;
-    const float inv_cap = a.cap != 0.0f ? 1.0f / a.cap : 0.0f;
-    const float unit = plain ? a.scale * kLog2e : 1.0f;  // scores to log2 units, where nothing has to be done to them
+    const float unit = plain ? scale * kLog2e : 1.0f;  // scores to log2 units, where nothing has to be done to them
 
     uint32_t t0 = part.start;
     const uint32_t end = part.end;  // steps [start, end) of 64 keys
@@ -209,21 +223,22 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
                 for (int b = 0; b < 2; ++b) {
                     const int row = 32 * b + j;
                     const u32x4 k = *reinterpret_cast<const u32x4*>(&sm.k[buf][row * DP + 8 * ((2 * c + h) ^ swap_k<CH>(j))]);
-                    s[b] = mma32<TC>(k, q[c], s[b]);
+#pragma unroll
+                    for (int p = NQ - 1; p >= 0; --p) s[b] = mma32<TC>(k, q[p][c], s[b]);
                 }
-            ahead_of_products<2 * KS, 1>();
+            ahead_of_products<2 * KS, 1, NQ>();
             const bool seen = there == ~uint64_t(0) && pos_first >= 0 && (last <= pos_first || last < prefix) &&
                               (a.window == 0 || pos_last - (int)t0 < a.window);
             if (!plain) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < 2; ++b) {
+                    float x[16];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float x = s[b][r] * a.scale;
-                        if (a.cap != 0.0f) x = a.cap * score_tanh<false>(x * inv_cap);
-                        if (a.slopes != nullptr) x -= slope * fabsf((float)(pos - ((int)t0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4)));
-                        s[b][r] = x * kLog2e;
-                    }
+                    for (int r = 0; r < 16; ++r) x[r] = s[b][r];
+                    form.apply(a, x, (float)(pos - (int)t0 - 32 * b - 4 * h), [](int r) { return 8 * (r / 4) + r % 4; });
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[b][r] = x[r];
+                }
             }
             if (!seen) {
                 const uint64_t see = visible(there, (int)t0, pos, prefix, a.window) >> (4 * h);
@@ -251,20 +266,32 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
                     for (int r = 0; r < 16; ++r) acc[d][r] *= f;
             }
             const float ref = m == kNegInf ? 0.0f : m;
-            u32x4 p[4];
+            u32x4 p[NP][4];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) {
-                    const float x = exp2_hw(__builtin_fmaf(s[b][r], unit, -ref)), y = exp2_hw(__builtin_fmaf(s[b][r + 1], unit, -ref));
+                    float x = exp2_hw(__builtin_fmaf(s[b][r], unit, -ref)), y = exp2_hw(__builtin_fmaf(s[b][r + 1], unit, -ref));
                     l += x + y;
-                    p[2 * b + r / 8][r % 8 / 2] = narrow2<TC>(x, y);
+#pragma unroll
+                    for (int c = 0; c < NP; ++c) {
+                        const uint32_t w = narrow2<TC>(x, y);
+                        p[c][2 * b + r / 8][r % 8 / 2] = w;
+                        if (c + 1 < NP) {
+                            x -= widen_half<TC>(w, 0);
+                            y -= widen_half<TC>(w, 1);
+                        }
+                    }
                 }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = mma32<TC>(read_v(buf, d, i), p[i], acc[d]);
-            ahead_of_products<4 * DB, 2>();
+                for (int d = 0; d < DB; ++d) {
+                    const u32x4 v = read_v(buf, d, i);
+#pragma unroll
+                    for (int c = NP - 1; c >= 0; --c) acc[d] = mma32<TC>(v, p[c][i], acc[d]);
+                }
+            ahead_of_products<4 * DB, 2, NP>();
         }
         if (more) arrive(is_key(t0 + kPromptKeys, rows_next), buf ^ 1);
         rows = rows_next;
@@ -297,24 +324,28 @@ __global__ __launch_bounds__(kAttnThreads, DP > 128 ? 1 : 2) void paged_prompt_k
     }
 }
 
-template <typename TC>
+template <typename TC, bool HIGH>
 int launch_prompt_of(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) {
     auto go = [&](auto kernel) { return launch(kernel, dim3(blocks), kAttnThreads, s, a, sp); };
     switch (a.head_dim) {
-    case 64: return go(paged_prompt_kernel<TC, 64, true>);
-    case 128: return go(paged_prompt_kernel<TC, 128, true>);
-    case 256: return go(paged_prompt_kernel<TC, 256, true>);
+    case 64: return go(paged_prompt_kernel<TC, 64, true, HIGH>);
+    case 128: return go(paged_prompt_kernel<TC, 128, true, HIGH>);
+    case 256: return go(paged_prompt_kernel<TC, 256, true, HIGH>);
     default:
-        return a.head_dim < 64    ? go(paged_prompt_kernel<TC, 64, false>)
-               : a.head_dim < 128 ? go(paged_prompt_kernel<TC, 128, false>)
-                                  : go(paged_prompt_kernel<TC, 256, false>);
+        return a.head_dim < 64    ? go(paged_prompt_kernel<TC, 64, false, HIGH>)
+               : a.head_dim < 128 ? go(paged_prompt_kernel<TC, 128, false, HIGH>)
+                                  : go(paged_prompt_kernel<TC, 256, false, HIGH>);
     }
 }
 
 }  // namespace
 
-int launch_prompt(const AttnArgs& a, unsigned blocks, const ChunkSplit& sp, hipStream_t s) {
-    return a.dtype == SPH_F16 ? launch_prompt_of<f16>(a, blocks, sp, s) : launch_prompt_of<bf16>(a, blocks, sp, s);
+int launch_prompt(const AttnArgs& a, int cache_dtype, unsigned blocks, const ChunkSplit& sp, hipStream_t s) {
+    auto of = [&](auto tc) {
+        using TC = decltype(tc);
+        return a.dtype == cache_dtype ? launch_prompt_of<TC, false>(a, blocks, sp, s) : launch_prompt_of<TC, true>(a, blocks, sp, s);
+    };
+    return cache_dtype == SPH_F16 ? of(f16{}) : of(bf16{});
 }
 
 }  // namespace sph

@@ -222,8 +222,9 @@ def paged_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor,
     """Attention of one new token per sequence, q [B, Hq, D], over the pages (as rope_kv_append_paged; the
     tokens' own keys are there already): softmax of scale * q.k (default D ** -0.5), capped by softcap * tanh(s /
     softcap), less slopes[h] (f32 [Hq]) times the distance, over the last `window` keys (0: all). Rows of
-    sequences of length 0 are zeros. workspace: paged_attention_workspace bytes of uint8 to reuse on one stream
-    (None: allocated for the call). `out` may be q."""
+    sequences of length 0 are zeros. workspace: uint8 memory to reuse from call to call on one stream,
+    paged_attention_workspace bytes of it (with less, the keys are split into fewer parts; None: allocated for the
+    call). `out` may be q."""
     return _native.paged_attention(q, kcache, vcache, seq_lens, block_table, scale, softcap, window, slopes, out,
                                    workspace, bad_page_flag)
 
@@ -243,7 +244,7 @@ def paged_attention_chunk(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.T
 
 def paged_attention_workspace(n_q_heads: int, n_kv_heads: int, n_seqs: int, max_pages: int, page_size: int, head_dim: int,
                               n_tokens: Optional[int] = None) -> int:
-    """Bytes of workspace of paged_attention at these sizes, or, given n_tokens, of paged_attention_chunk."""
+    """The most bytes of workspace that paged_attention uses at these sizes, or, given n_tokens, paged_attention_chunk."""
     if n_tokens is None:
         n = lib().sph_paged_attention_workspace(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim)
     else:

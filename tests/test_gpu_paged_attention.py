@@ -97,6 +97,15 @@ def test_a_used_workspace_leaves_nothing(dev):
     for lens in ([333], [1, 333, 0, 16, 129], [700, 3, 650] * 5):
         c = Batch(14, 2, 64, lens=lens, seed=7)
         n = ops.paged_attention_workspace(14, 2, len(lens), c.table.shape[1], 16, 64)
-        ws = torch.full((n // 4 + 1,), float("nan"), device=dev).view(torch.uint8)
-        say("workspace", lens[:5])
-        check(ops.paged_attention(*c.to(dev), workspace=ws), c, "workspace", weights(F16, F16, False))
+        for size in (n, n // 3, n // 40, 0):  # with less of it the keys are split less
+            ws = torch.full((size // 4 + 4,), float("nan"), device=dev).view(torch.uint8)[:size]
+            say("workspace", lens[:5], size)
+            check(ops.paged_attention(*c.to(dev), workspace=ws), c, "workspace", weights(F16, F16, False))
+    for lens, new in (([700], [9]), ([1300, 40, 600], [33, 40, 1])):
+        c = Batch(14, 2, 64, lens=lens, new=new, seed=8)
+        n = ops.paged_attention_workspace(14, 2, len(lens), c.table.shape[1], 16, 64, n_tokens=c.q.shape[0])
+        assert n > 0
+        for size in (n, n // 2, 0):
+            ws = torch.full((size // 4 + 4,), float("nan"), device=dev).view(torch.uint8)[:size]
+            say("workspace, chunk", lens, size)
+            check(ops.paged_attention_chunk(*c.to(dev), workspace=ws), c, "workspace", weights(F16, F16, True))
