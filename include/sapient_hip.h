@@ -358,7 +358,8 @@ int sph_kv_cache_update_into(const void* src, int src_dtype, const void* cache, 
  * from the cache for such a position, and a key there takes no part.
  * The layout is the contiguous cache's with pages as its outer axis: a [n_kv,
  * max_seq, head_dim] cache is a pool of one page of max_seq tokens.
- * page_size >= 1 and any n_pages with n_pages · n_kv_heads · page_size < 2^32 - 1. */
+ * page_size >= 1, any n_pages with n_pages · n_kv_heads · page_size < 2^32 - 1,
+ * sequences of up to 2^30 tokens. */
 
 /* sph_rope_kv_append_tokens into a paged cache: q (rotated, into q_out, which is
  * token-major here and may be q itself), k (rotated) and v of every new token,
@@ -383,7 +384,9 @@ int sph_rope_kv_append_paged(const void* q, void* q_out, int64_t n_q_heads, cons
  *   s = scale · q·k;  softcap > 0: s = softcap · tanh(s / softcap);
  *   slopes (device f32 [n_q_heads], optional): s = s - slopes[h] · |P - p|;
  * window > 0: only keys with P - p < window take part (0: all). out = sum of
- * softmax(s) · v; a row without keys is zeros. Replaces the decode form of
+ * softmax(s) · v; a row without keys is zeros. A value of v that is not finite
+ * leaves the rows that see its key not finite, in its channel at least, and no
+ * other row; what lies in a page past a sequence's end reaches nothing. Replaces the decode form of
  * WgpuContext::attention (crates/sapient-backends/wgpu/src/resident.rs, shader
  * attention.wgsl, grouped query heads), which the decode engine takes as a callback.
  * dtype ∈ {F32, F16, BF16} for q and out; cache_dtype ∈ {F32, F16, BF16};

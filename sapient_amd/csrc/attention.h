@@ -235,6 +235,16 @@ struct Tile {
     int pos0;                       // position of the sequence's first new token
 };
 
+// Whether a word of V (an f32, or two values of a half type) holds what is not finite. In a step of keys that only some of
+// a tile's rows see, such a value would reach the others as 0 · inf: there it is cleared, and its key's score made NaN in
+// the rows that see the key.
+template <typename TC>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+    if constexpr (sizeof(TC) == 4) return (w & 0x7F800000u) == 0x7F800000u;
+    constexpr uint32_t ones = __is_same(TC, f16) ? 0x7C007C00u : 0x7F807F80u, one = __is_same(TC, f16) ? 0x04000400u : 0x00800080u;
+    return (((w & ones) + one) & 0x80008000u) != 0u;
+}
+
 // HIGH: q is f32, or the cache's type is another one than q's. LOW: both the same half type.
 template <typename TC, int DP, bool EXACT, bool HIGH>
 struct TileKernel {
@@ -270,7 +280,8 @@ struct TileKernel {
 
     // The keys [lo, hi) of the tile, over the block's four waves; then store(column, channel, m, l, sums of 4 channels)
     // for every column of the tile, by the block's threads.
-    template <typename Store>
+    // MIXED: the tile's columns may see different keys.
+    template <bool MIXED, typename Store>
     __device__ __forceinline__ void attend(const AttnArgs& a, Shared& sm, const Tile& t, uint32_t lo, uint32_t hi, Store store) {
         const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, j = lane % 16, g = lane / 16;
         const int D = EXACT ? DP : a.head_dim;
@@ -432,13 +443,6 @@ struct TileKernel {
 #pragma unroll
                 for (int i = 0; i < 4 * KB; ++i) s[i / 4][i % 4] = x[i];
             }
-            if (!seen) {
-                const uint32_t see = (uint32_t)visible(there, (int)t0, pos, prefix, a.window) >> (4 * g);
-#pragma unroll
-                for (int b = 0; b < KB; ++b)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[b][r] = see & (1u << (16 * b + r)) ? s[b][r] : kNegInf;
-            }
             if (!whole) {  // what lies in a row that is no key of the sequence may be anything, and 0 · inf is not 0
 #pragma unroll
                 for (int e = 0; e < VT; ++e)
@@ -448,6 +452,31 @@ struct TileKernel {
                     }
             }
 
+            if (!seen) {
+                const uint32_t see = (uint32_t)visible(there, (int)t0, pos, prefix, a.window) >> (4 * g);
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[b][r] = see & (1u << (16 * b + r)) ? s[b][r] : kNegInf;
+                if constexpr (MIXED) {
+                    uint32_t odd = 0;  // this lane's keys with a value that is not finite, as bits of see
+#pragma unroll
+                    for (int e = 0; e < VT; ++e) {
+                        bool any = false;
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) {
+                            const bool x = not_finite<TC>(v[e][w]);
+                            any |= x;
+                            v[e][w] = x ? 0u : v[e][w];
+                        }
+                        if ((__ballot(any) >> (16 * g)) & 0xFFFF) odd |= 1u << (16 * (e / 4) + e % 4);
+                    }
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[b][r] = see & odd & (1u << (16 * b + r)) ? __builtin_nanf("") : s[b][r];
+                }
+            }
             float top = s[0][0];
 #pragma unroll
             for (int b = 0; b < KB; ++b)
@@ -597,9 +626,9 @@ __device__ __forceinline__ bool chunk_tile(const AttnArgs& a, const ChunkSplit& 
     t.row0 = begin;
     t.rows = (end - begin) * a.group;
     t.first = ROWS * (int)tile;
-    t.pos0 = a.pages.lens[t.seq] - (end - begin);
-    if (t.pos0 < 0 && threadIdx.x == 0 && a.bad != nullptr) *a.bad = 1;
-    const int keys = a.pages.keys(t.seq, a.bad, threadIdx.x == 0);
+    const int len = a.pages.length(t.seq), keys = len < a.pages.capacity ? len : a.pages.capacity;
+    t.pos0 = len - (end - begin);
+    if ((t.pos0 < 0 || keys < len) && threadIdx.x == 0 && a.bad != nullptr) *a.bad = 1;
 
     // The keys that any of the tile's rows may see.
     const int last_col = t.first + ROWS - 1 < t.rows ? t.first + ROWS - 1 : t.rows - 1;
@@ -632,14 +661,14 @@ __global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_tiles_ker
     };
     K k;
     if (sp.splits == 1) {
-        k.attend(a, sm, t, lo, hi, [&](int c, int d, float, float l, f32x4 sum) {
+        k.template attend<true>(a, sm, t, lo, hi, [&](int c, int d, float, float l, f32x4 sum) {
             const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] = l == 0.0f ? 0.0f : sum[i] * f;
             store4_from_f32(a.out, a.dtype, row_of(c) * (size_t)a.head_dim + d, sum);
         });
     } else {
-        k.attend(a, sm, t, lo, hi, [&](int c, int d, float m, float l, f32x4 sum) {
+        k.template attend<true>(a, sm, t, lo, hi, [&](int c, int d, float m, float l, f32x4 sum) {
             chunk_part_sum(a, sp, part.split, row_of(c), d, sum);
             if (d == 0) chunk_part_ml(a, sp, part.split, row_of(c), m, l);
         });
@@ -718,8 +747,8 @@ struct SplitRange {
     int len;
     uint32_t lo, hi, start, steps;
     __device__ __forceinline__ SplitRange(const AttnArgs& a, int b) {
-        len = a.pages.lens[b];
-        hi = len < 0 ? 0u : (uint32_t)(len < a.pages.capacity ? len : a.pages.capacity);
+        len = a.pages.length(b);
+        hi = (uint32_t)(len < a.pages.capacity ? len : a.pages.capacity);
         lo = a.window > 0 && len > a.window ? (uint32_t)(len - a.window) : 0u;
         if (lo > hi) lo = hi;
         start = lo & ~31u;
@@ -775,7 +804,7 @@ __global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_split_ker
             }
             K k;
             if (n == r.steps) {
-                k.attend(a, sm, t, lo, hi, [&](int c, int d, float, float l, f32x4 sum) {
+                k.template attend<false>(a, sm, t, lo, hi, [&](int c, int d, float, float l, f32x4 sum) {
                     const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sum[i] = l == 0.0f ? 0.0f : sum[i] * f;
@@ -784,7 +813,7 @@ __global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_split_ker
                 });
             } else {
                 const size_t slot = 2 * (size_t)share + (u == begin ? 0 : 1);
-                k.attend(a, sm, t, lo, hi, [&](int c, int d, float m, float l, f32x4 sum) {
+                k.template attend<false>(a, sm, t, lo, hi, [&](int c, int d, float m, float l, f32x4 sum) {
                     const size_t row = slot * (size_t)sp.cols + (size_t)c;
                     *reinterpret_cast<f32x4*>(sp.part + row * (size_t)a.head_dim + d) = sum;
                     if (d == 0) {
@@ -815,7 +844,7 @@ __global__ __launch_bounds__(kAttnThreads, K::kBlocksPerCu) void paged_whole_ker
     t.rows = a.group;
     t.pos0 = r.len - 1;
     K k;
-    k.attend(a, sm, t, r.lo, r.hi, [&](int c, int d, float, float l, f32x4 sum) {
+    k.template attend<false>(a, sm, t, r.lo, r.hi, [&](int c, int d, float, float l, f32x4 sum) {
         const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] = l == 0.0f ? 0.0f : sum[i] * f;

@@ -58,6 +58,7 @@ template <typename TC, int DP>
 struct PromptShared {
     alignas(16) uint16_t k[2][kPromptKeys * DP];
     alignas(16) uint16_t v[2][kPromptKeys * DP];
+    uint64_t odd[2][kAttnWaves];  // the keys of each buffer whose V had a value that is not finite (of edge steps), by finder
     Located located;
 };
 
@@ -150,14 +151,35 @@ __global__ __launch_bounds__(kAttnThreads, prompt_blocks(DP, HIGH)) void paged_p
             if (EXACT || dv < D) to_lds(vc + at + dv, &sm.v[buf][to]);
         }
     };
-    auto arrive = [&](uint64_t there, int buf) {
+    // Whether all the block's rows see all of the step's keys.
+    const int block_first = t.pos0 + t.first / a.group;
+    const int block_last = t.pos0 + ((t.first + kPromptRows < t.rows ? t.first + kPromptRows : t.rows) - 1) / a.group;
+    auto all_see = [&](uint64_t there, int t0) {
+        const int last = t0 + kPromptKeys - 1;
+        return there == ~uint64_t(0) && block_first >= 0 && (last <= block_first || last < prefix) &&
+               (a.window == 0 || block_last - t0 < a.window);
+    };
+    auto arrive = [&](uint64_t there, uint32_t t0, int buf) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (there == ~uint64_t(0)) return;
+        uint64_t odd = 0;
+        if (!all_see(there, (int)t0)) {
+#pragma unroll 1
+            for (int i = 0; i < PL; ++i) {
+                const int piece = i * kAttnThreads + tid;
+                u32x4* p = reinterpret_cast<u32x4*>(&sm.v[buf][8 * piece]);
+                const u32x4 w = *p;
+                const bool key = (there >> (piece / CH)) & 1;
+                if (!key || not_finite<TC>(w[0]) || not_finite<TC>(w[1]) || not_finite<TC>(w[2]) || not_finite<TC>(w[3])) {
+                    *p = u32x4{0, 0, 0, 0};
+                    if (key) odd |= uint64_t(1) << (piece / CH);
+                }
+            }
+            if (__any(odd != 0)) {
 #pragma unroll
-        for (int i = 0; i < PL; ++i) {
-            const int piece = i * kAttnThreads + tid;
-            if (!((there >> (piece / CH)) & 1)) *reinterpret_cast<u32x4*>(&sm.v[buf][8 * piece]) = u32x4{0, 0, 0, 0};
+                for (int d = 1; d < kWave; d <<= 1) odd |= __shfl_xor(odd, d);
+            }
         }
+        if (lane == 0) sm.odd[buf][wave] = odd;
     };
     if constexpr (!EXACT) {
         for (int i = tid; i < 2 * kPromptKeys * CH; i += kAttnThreads) {
@@ -197,7 +219,7 @@ __global__ __launch_bounds__(kAttnThreads, prompt_blocks(DP, HIGH)) void paged_p
         id_next = entry_at(t0 + kPromptKeys);
         rows = row_at(t0, id);
         load_step(rows, 0);
-        arrive(is_key(t0, rows), 0);
+        arrive(is_key(t0, rows), t0, 0);
     }
     __syncthreads();
     for (int buf = 0; t0 < end; t0 += kPromptKeys, buf ^= 1) {
@@ -227,8 +249,7 @@ __global__ __launch_bounds__(kAttnThreads, prompt_blocks(DP, HIGH)) void paged_p
                     for (int p = NQ - 1; p >= 0; --p) s[b] = mma32<TC>(k, q[p][c], s[b]);
                 }
             ahead_of_products<2 * KS, 1, NQ>();
-            const bool seen = there == ~uint64_t(0) && pos_first >= 0 && (last <= pos_first || last < prefix) &&
-                              (a.window == 0 || pos_last - (int)t0 < a.window);
+            const bool seen = all_see(there, (int)t0);
             if (!plain) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
@@ -247,6 +268,14 @@ __global__ __launch_bounds__(kAttnThreads, prompt_blocks(DP, HIGH)) void paged_p
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         s[b][r] = (uint32_t)(see >> (32 * b)) & (1u << (8 * (r / 4) + r % 4)) ? s[b][r] : kNegInf;
+                const uint64_t odd = (sm.odd[buf][0] | sm.odd[buf][1] | sm.odd[buf][2] | sm.odd[buf][3]) >> (4 * h) & see;
+                if (__any(odd != 0)) {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            s[b][r] = (uint32_t)(odd >> (32 * b)) & (1u << (8 * (r / 4) + r % 4)) ? __builtin_nanf("") : s[b][r];
+                }
             }
             float top = s[0][0];
 #pragma unroll
@@ -293,7 +322,7 @@ __global__ __launch_bounds__(kAttnThreads, prompt_blocks(DP, HIGH)) void paged_p
                 }
             ahead_of_products<4 * DB, 2, NP>();
         }
-        if (more) arrive(is_key(t0 + kPromptKeys, rows_next), buf ^ 1);
+        if (more) arrive(is_key(t0 + kPromptKeys, rows_next), t0 + kPromptKeys, buf ^ 1);
         rows = rows_next;
         __syncthreads();
     }

@@ -14,6 +14,7 @@
 namespace sph {
 
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+constexpr int kMaxTokens = 1 << 30;  // of a sequence: positions and steps past them stay in 32 bits
 
 // n / d for n < 2^31 by a multiplication (page sizes are arguments; a division by one is some forty operations):
 // with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(m, n) + n) >> s, and for n < 2^31
@@ -39,7 +40,7 @@ struct PagedTable {
     // Pool row of token t (kv head 0; head h's is h · page_size further), or kNoRow.
     __device__ __forceinline__ uint32_t row(int seq, uint32_t t) const {
         const uint32_t p = page.quotient(t);
-        if (p >= (uint32_t)max_pages) return kNoRow;
+        if (p >= (uint32_t)max_pages || t >= (uint32_t)kMaxTokens) return kNoRow;
         const uint32_t id = (uint32_t)table[(size_t)seq * (size_t)max_pages + p];
         return id < (uint32_t)n_pages ? id * (uint32_t)n_kv * page.d + (t - p * page.d) : kNoRow;
     }
@@ -52,13 +53,7 @@ struct PagedTable {
         return id < (uint32_t)n_pages ? id * (uint32_t)n_kv * page.d + (t - page.quotient(t) * page.d) : kNoRow;
     }
 
-    // Keys of sequence b that the table can name: its length, cut at the capacity (and then flagged, by one lane).
-    __device__ __forceinline__ int keys(int b, int32_t* bad, bool tell) const {
-        const int len = lens[b];
-        if (len <= capacity) return len < 0 ? 0 : len;
-        if (bad != nullptr && tell) *bad = 1;
-        return capacity;
-    }
+    __device__ __forceinline__ int length(int b) const { return lens[b] < 0 ? 0 : lens[b]; }
 
     // The rows [begin, end) of sequence b's new tokens among n_rows, whatever cu holds.
     __device__ __forceinline__ void new_rows(int b, int n_rows, int& begin, int& end) const {
@@ -97,7 +92,7 @@ inline PagedTable paged_table(const int32_t* seq_lens, const int32_t* cu_q, cons
     p.n_kv = (int)n_kv;
     p.page = Divisor((uint32_t)page_size);
     const int64_t capacity = max_pages * page_size;
-    p.capacity = capacity < INT32_MAX ? (int)capacity : INT32_MAX;
+    p.capacity = capacity < kMaxTokens ? (int)capacity : kMaxTokens;
     return p;
 }
 

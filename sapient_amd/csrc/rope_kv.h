@@ -187,11 +187,14 @@ __device__ __forceinline__ void load_angles(const float* p, float (&ag)[2 * P]) 
 //
 // A paged cache (Args::kPaged) differs in where a token's position and its cache
 // row come from. Row s belongs to the sequence b with cu[b] <= s < cu[b + 1]
-// (b = s where there is one token each): the block counts the cu entries at
-// or below its first row, each thread one entry (requested ahead of the rows,
-// so that waiting for it does not wait for them), and its other rows walk on from
-// there. The position is lens[b] - (cu[b + 1] - s); the table's entry is
-// requested as soon as it is known and arrives behind the angles.
+// (b = s where there is one token each). Up to 64 sequences a wave's lanes hold
+// one's cu[b + 1] and length each (requested ahead of the rows, so that waiting
+// for them does not wait for those), count the entries at or below the block's
+// first row, and walk on to their own rows' by exchanges between lanes, with no
+// further load (a prefill step of 6 prompts, 8513 tokens of 32 + 8 x 128 f16:
+// 44.8 -> 41.1 us, 35 for one contiguous cache); more sequences are counted by the block. The position is
+// lens[b] - (cu[b + 1] - s); the table's entry is requested as soon as it is
+// known and arrives behind the angles.
 template <typename Args, int P, bool INTERLEAVED, bool TM, int U, bool BIAS, bool NT>
 __global__ __launch_bounds__(kThreads) void rope_kv_kernel(Args a) {
     using T = typename Args::Q;
@@ -220,11 +223,14 @@ __global__ __launch_bounds__(kThreads) void rope_kv_kernel(Args a) {
     constexpr bool kOwn = P == 1;  // a thread's one angle: no exchange (3 tokens of 14 + 2 x 64: 2.87 -> 2.66 us)
     // Clamped, not predicated: a load in a branch is waited for at its end where its value is converted there.
     auto pos_at = [&](int64_t t) { return a.pos[t < a.seq ? t : a.seq - 1]; };
-    int32_t ps = 0, cu_word = INT32_MAX;
+    int32_t ps = 0, cu_word = INT32_MAX, len_word = 0, cu_first = 0;
     if constexpr (!Args::kPaged) {
         ps = pos_at(s);
     } else if (a.pages.cu != nullptr) {
-        cu_word = a.pages.cu[1 + (tid < a.pages.n_seqs ? tid : a.pages.n_seqs - 1)];
+        const int n = a.pages.n_seqs, i = n <= kWave ? tid % kWave : tid, at = i < n ? i : n - 1;
+        cu_word = a.pages.cu[1 + at];
+        len_word = a.pages.lens[at];
+        cu_first = a.pages.cu[0];
     } else {
         ps = a.pages.lens[s < a.seq ? s : a.seq - 1] - 1;
     }
@@ -282,31 +288,53 @@ __global__ __launch_bounds__(kThreads) void rope_kv_kernel(Args a) {
         if (a.pages.cu != nullptr) {
             __shared__ int counted[kThreads / kWave];
             const int n = a.pages.n_seqs;
-            int below = 0;  // cu entries at or below the block's first row
-            for (int i = tid; i < n; i += blockDim.x) {
-                if (i >= (int)blockDim.x) cu_word = a.pages.cu[1 + i];
-                below += cu_word <= s0;
-            }
-#pragma unroll
-            for (int m = 32; m > 0; m >>= 1) below += __shfl_xor(below, m);
-            if (tid % kWave == 0) counted[tid / kWave] = below;
-            __syncthreads();
-            int first = 0;
-            for (int w = 0; w < (int)blockDim.x / kWave; ++w) first += counted[w];
-            auto locate = [&](int64_t t, int& b) {  // the sequence and the position of row t
-                b = first;
-                while (b < n && a.pages.cu[1 + b] <= t) ++b;
-                if (b >= n || t >= a.seq || a.pages.cu[b] > t) {
-                    b = n;
-                    return -1;
+            if (n <= kWave) {
+                const int first = __popcll(__ballot(tid % kWave < n && cu_word <= s0));
+                auto locate = [&](int64_t t, int& b) {  // by all lanes of the wave
+                    b = first;
+                    int32_t next;
+                    for (;;) {
+                        next = __shfl(cu_word, b);
+                        const bool on = t < a.seq && b < n && next <= t;
+                        if (!__any(on)) break;
+                        b += on;
+                    }
+                    const int64_t p = (int64_t)__shfl(len_word, b) - (next - t);
+                    if (t >= a.seq || t < cu_first) b = n;
+                    return b >= n || p < 0 ? -1 : (int)p;
+                };
+                ps = locate(s, seq_of);
+                if constexpr (!kOwn) {
+                    int b;
+                    apos = locate(s0 + tk, b);
                 }
-                const int64_t p = a.pages.lens[b] - (a.pages.cu[b + 1] - t);
-                return p < 0 ? -1 : (int)p;
-            };
-            ps = locate(s, seq_of);
-            if constexpr (!kOwn) {
-                int b;
-                apos = locate(s0 + tk, b);
+            } else {
+                int below = 0;  // cu entries at or below the block's first row
+                for (int i = tid; i < n; i += blockDim.x) {
+                    if (i >= (int)blockDim.x) cu_word = a.pages.cu[1 + i];
+                    below += cu_word <= s0;
+                }
+#pragma unroll
+                for (int m = 32; m > 0; m >>= 1) below += __shfl_xor(below, m);
+                if (tid % kWave == 0) counted[tid / kWave] = below;
+                __syncthreads();
+                int first = 0;
+                for (int w = 0; w < (int)blockDim.x / kWave; ++w) first += counted[w];
+                auto locate = [&](int64_t t, int& b) {  // the sequence and the position of row t
+                    b = first;
+                    while (b < n && a.pages.cu[1 + b] <= t) ++b;
+                    if (b >= n || t >= a.seq || a.pages.cu[b] > t) {
+                        b = n;
+                        return -1;
+                    }
+                    const int64_t p = a.pages.lens[b] - (a.pages.cu[b + 1] - t);
+                    return p < 0 ? -1 : (int)p;
+                };
+                ps = locate(s, seq_of);
+                if constexpr (!kOwn) {
+                    int b;
+                    apos = locate(s0 + tk, b);
+                }
             }
         }
         if (active && ps >= 0) crow0 = a.pages.row(seq_of, (uint32_t)ps);
