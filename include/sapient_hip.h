@@ -391,7 +391,8 @@ int sph_rope_kv_append_paged(const void* q, void* q_out, int64_t n_q_heads, cons
  * attention.wgsl, grouped query heads), which the decode engine takes as a callback.
  * dtype ∈ {F32, F16, BF16} for q and out; cache_dtype ∈ {F32, F16, BF16};
  * head_dim a multiple of 8, at most 256; q, out, kcache and vcache 16-byte
- * aligned; n_q_heads a multiple of n_kv_heads; scale finite. Sums and
+ * aligned; n_q_heads a multiple of n_kv_heads; scale finite, softcap 0 or at least
+ * 1e-6. Sums and
  * softmax statistics are f32. workspace: device memory, 16-byte aligned, of one
  * call at a time (calls of one stream may share it, and graphs replayed in one),
  * whose contents do not matter before or after: with sph_paged_attention_workspace

@@ -15,7 +15,8 @@ int attn_args(AttnArgs& a, const void* q, void* out, int64_t n_q_heads, int64_t 
     if (n_q_heads < 1 || n_q_heads > INT32_MAX || n_q_heads % n_kv_heads != 0) return SPH_EINVAL;
     if (head_dim <= 0 || head_dim % 8 != 0 || head_dim > 256) return SPH_EINVAL;
     if (n_rows * n_q_heads > INT32_MAX) return SPH_EINVAL;
-    if (!isfinite(scale) || !isfinite(softcap) || softcap < 0.0f || window < 0) return SPH_EINVAL;
+    if (!isfinite(scale) || !isfinite(softcap) || window < 0) return SPH_EINVAL;
+    if (softcap != 0.0f && !(softcap >= 1e-6f)) return SPH_EINVAL;  // scale / softcap stays finite
     if (!aligned(cu_q, 4) || !aligned(slopes, 4) || !aligned(prefix_lens, 4)) return SPH_EINVAL;
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(kcache, 16) || !aligned(vcache, 16)) return SPH_EINVAL;
     if (n_rows > 0 && n_seqs > 0 && (q == nullptr || out == nullptr || kcache == nullptr || vcache == nullptr)) return SPH_EINVAL;

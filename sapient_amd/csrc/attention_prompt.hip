@@ -5,12 +5,18 @@
 // for the whole group) share steps of 64 keys through LDS, on 32x32x16 matrix instructions. Scores are transposed
 // (S^T = K Q^T) as in the 16-column kernel: lane (j = lane % 32, h = lane / 32) holds column j's scores of tokens 8b +
 // 4h + 0..3, which is the order in which it feeds them back as the second operand, so weights never leave their lane.
-// Both lie in LDS as they come, rows of DP channels in 16-byte pieces, piece c of row r at c ^ swap(r), so that what a
+// K and V lie in LDS as they come, rows of DP channels in 16-byte pieces, piece c of row r at c ^ swap(r), so that what a
 // read touches at once (a piece of 8 and of 16 neighbouring rows of K; of V, 32 bytes of 4 neighbouring rows, and 64) lies
 // in different banks. They go there straight from
 // memory (16 bytes a lane; a wave's lanes fill 1 KB in a row, so the swap is in which piece a lane asks for), into the
 // other of two buffers while a step is computed: no registers hold them, no instruction moves them. V is read
 // transposed (ds_read_b64_tr_b16: of 4 rows by 16 channels, a channel's 4 values to a lane). One barrier a step.
+//
+// What bounds it: per step and wave 32 products of 32 cycles and some 240 vector instructions (of which 32 exponentials),
+// and the two waves of a SIMD hardly overlap them: matrix cores busy 41 % of the time, vector units 46 %. Ragged prompts of
+// 10033 tokens, 32 + 8 heads x 128 bf16: 331 to 345 us by machine, 880 TFLOP/s of the products that the masks leave (a
+// library product of 8192^3 1340). By step: K and V through registers 423, straight to LDS 368, reads ahead 358, swapped
+// pieces 331; raised wave priority around the products, and scalar addresses, gained nothing.
 #include "attention.h"
 
 namespace sph {

@@ -196,7 +196,7 @@ __device__ __forceinline__ void load_angles(const float* p, float (&ag)[2 * P]) 
 // lens[b] - (cu[b + 1] - s); the table's entry is requested as soon as it is
 // known and arrives behind the angles.
 template <typename Args, int P, bool INTERLEAVED, bool TM, int U, bool BIAS, bool NT>
-__global__ __launch_bounds__(kThreads) void rope_kv_kernel(Args a) {
+__device__ __forceinline__ void rope_kv_step(Args a) {
     using T = typename Args::Q;
     static_assert(TM || !Args::kPaged, "a paged append reads the projections' layout");
     __shared__ uint32_t inv_pio4[24];
@@ -442,6 +442,15 @@ inline void fill_dens(DenTable& den, int half, int rotary_dim, float base) {
         den.v[i] = i < half ? powf(base, 2.0f * (float)i / (float)rotary_dim) : 1.0f;
 }
 
+template <typename T, typename TC, int P, bool INTERLEAVED, bool TM, int U, bool BIAS, bool NT>
+__global__ __launch_bounds__(kThreads) void rope_kv_kernel(RopeKvArgs<T, TC> a) {
+    rope_kv_step<RopeKvArgs<T, TC>, P, INTERLEAVED, TM, U, BIAS, NT>(a);
+}
+template <typename T, typename TC, int P, bool INTERLEAVED, int U, bool BIAS, bool NT>
+__global__ __launch_bounds__(kThreads) void rope_kv_paged_kernel(RopeKvPagedArgs<T, TC> a) {
+    rope_kv_step<RopeKvPagedArgs<T, TC>, P, INTERLEAVED, true, U, BIAS, NT>(a);
+}
+
 // Launch shape, from the lanes that the rows need (one row per thread and pass):
 //  - small (up to 2^14: decode steps): blocks of one wave, so that the rows spread over the CUs, each with the
 //    angles of one token (two heads a block 2.96 us, four 3.14, one 3.00 at one token of 14 + 2 heads x 64; with
@@ -498,8 +507,12 @@ int launch_rope_kv_p(A& a, hipStream_t stream) {
             const int64_t toks = a.seq - a.s_first < most ? a.seq - a.s_first : most;
             const dim3 grid((unsigned)((toks + a.toks - 1) / a.toks), (unsigned)(tiles < kMaxY ? tiles : kMaxY));
             auto go = [&](auto u, auto b, auto n) {
-                return launch(rope_kv_kernel<A, P, IL, TM, decltype(u)::value, decltype(b)::value, decltype(n)::value>,
-                              grid, threads, stream, a);
+                if constexpr (A::kPaged)
+                    return launch(rope_kv_paged_kernel<T, TC, P, IL, decltype(u)::value, decltype(b)::value, decltype(n)::value>,
+                                  grid, threads, stream, a);
+                else
+                    return launch(rope_kv_kernel<T, TC, P, IL, TM, decltype(u)::value, decltype(b)::value, decltype(n)::value>,
+                                  grid, threads, stream, a);
             };
             using std::false_type;
             using std::true_type;

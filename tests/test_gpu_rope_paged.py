@@ -134,3 +134,22 @@ def test_bad_pages_write_nothing_and_raise_the_flag(dev, new):
         assert int(s.flag) == 1
         # four of the five rows have a position; the first has none and stays
         assert (got[s.starts[3]] == 7).all() and not (got[s.starts[3] + 1:] == 7).all()
+
+
+@pytest.mark.parametrize("cu", [[0, 0, 0], [5, 9, 9], [0, 9, 3], [-4, 2, 50], [9, 4, 0], [7, 7, 7]], ids=str)
+@pytest.mark.parametrize("many", [False, True])
+def test_any_cu_q_stays_in_bounds(dev, cu, many):
+    """Nothing outside q_out and the pools is touched, whatever cu_q holds, and rows outside every sequence stay."""
+    lens = [40, 30] + [0] * (100 if many else 0)
+    s = Step(dev, 8, 2, 64, lens, [4, 5] + [0] * (len(lens) - 2), F16, F16, 16)
+    cu = cu + [cu[-1]] * (len(lens) - 2)
+    s.cu = torch.tensor(cu, dtype=torch.int32, device=dev)
+    guard = torch.full((s.q.shape[0] + 8, 8, 64), 7.0, dtype=F16, device=dev)
+    print("case", cu[:4], many, flush=True)
+    got, kc, vc = s.run(out=guard[4:-4])
+    assert (guard[:4] == 7).all() and (guard[-4:] == 7).all()
+    if cu == sorted(cu):
+        inside = torch.zeros(got.shape[0], dtype=torch.bool)
+        for a, b in zip(cu, cu[1:]):
+            inside[max(a, 0):max(0, min(b, got.shape[0]))] = True
+        assert (got.cpu()[~inside] == 7).all()
