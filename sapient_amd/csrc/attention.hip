@@ -4,6 +4,17 @@
 #include <math.h>
 
 namespace sph {
+namespace {
+
+// Sizes that every count of rows, tiles and keys stays in 32 bits for.
+bool sizes_ok(int64_t nq, int64_t nkv, int64_t n_seqs, int64_t max_pages, int64_t page_size, int64_t head_dim, int64_t n_rows) {
+    if (nkv < 1 || nq < 1 || nq > INT32_MAX || nkv > INT32_MAX || nq % nkv != 0) return false;
+    if (head_dim <= 0 || head_dim % 8 != 0 || head_dim > 256) return false;
+    if (n_seqs < 0 || n_seqs > INT32_MAX || max_pages < 0 || max_pages > INT32_MAX || page_size < 1 || page_size > INT32_MAX) return false;
+    return n_rows >= 0 && n_rows <= INT32_MAX && n_rows * nq <= INT32_MAX - kPromptRows;
+}
+
+}  // namespace
 
 int attn_args(AttnArgs& a, const void* q, void* out, int64_t n_q_heads, int64_t n_kv_heads, int dtype, const int32_t* cu_q,
               const int32_t* seq_lens, const int32_t* block_table, int64_t n_seqs, int64_t max_pages, int64_t n_rows,
@@ -12,9 +23,7 @@ int attn_args(AttnArgs& a, const void* q, void* out, int64_t n_q_heads, int64_t 
               const int32_t* prefix_lens, int32_t* bad) {
     if (!is_float_dtype(dtype) || !is_float_dtype(cache_dtype)) return SPH_EINVAL;
     if (!paged_ok(seq_lens, block_table, n_seqs, max_pages, n_pages, page_size, n_kv_heads, n_rows)) return SPH_EINVAL;
-    if (n_q_heads < 1 || n_q_heads > INT32_MAX || n_q_heads % n_kv_heads != 0) return SPH_EINVAL;
-    if (head_dim <= 0 || head_dim % 8 != 0 || head_dim > 256) return SPH_EINVAL;
-    if (n_rows * n_q_heads > INT32_MAX) return SPH_EINVAL;
+    if (!sizes_ok(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, n_rows)) return SPH_EINVAL;
     if (!isfinite(scale) || !isfinite(softcap) || window < 0) return SPH_EINVAL;
     if (softcap != 0.0f && !(softcap >= 1e-6f)) return SPH_EINVAL;  // scale / softcap stays finite
     if (!aligned(cu_q, 4) || !aligned(slopes, 4) || !aligned(prefix_lens, 4)) return SPH_EINVAL;
@@ -187,18 +196,14 @@ extern "C" int sph_paged_attention_chunk(const void* q, void* out, int64_t n_q_h
 
 extern "C" int64_t sph_paged_attention_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_pages,
                                                  int64_t page_size, int64_t head_dim) {
-    if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads != 0 || n_seqs < 0 || max_pages < 0 || page_size < 1 ||
-        head_dim < 1 || head_dim > 256)
-        return SPH_EINVAL;
+    if (!sph::sizes_ok(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, n_seqs)) return SPH_EINVAL;
     return sph::split_plan(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, 0, INT64_MAX).bytes;
 }
 
 extern "C" int64_t sph_paged_attention_chunk_workspace(int64_t n_q_heads, int64_t n_kv_heads, int64_t n_seqs,
                                                        int64_t max_pages, int64_t page_size, int64_t n_tokens,
                                                        int64_t head_dim) {
-    if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads != 0 || n_seqs < 0 || max_pages < 0 || page_size < 1 ||
-        head_dim < 1 || head_dim > 256 || n_tokens < 0)
-        return SPH_EINVAL;
+    if (!sph::sizes_ok(n_q_heads, n_kv_heads, n_seqs, max_pages, page_size, head_dim, n_tokens)) return SPH_EINVAL;
     // The larger of the two tiles' plans.
     int64_t most = 0;
     for (const bool prompt : {false, true}) {

@@ -90,8 +90,11 @@ def test_workspace_sizes(L):
     assert ops.paged_attention_workspace(32, 8, 64, 32, 16, 128) == 0       # tables of 512 keys are not split
     assert ops.paged_attention_workspace(32, 8, 1, 512, 16, 128, n_tokens=8192) == 0  # enough tiles
     assert ops.paged_attention_workspace(32, 8, 1, 512, 16, 128, n_tokens=8) > 0
-    with pytest.raises(_lib.SapientHipError):
-        ops.paged_attention_workspace(7, 2, 1, 1, 16, 64)
+    for bad in ((7, 2, 1, 1, 16, 64), (8, 2, 1 << 31, 1, 16, 64), (8, 2, 1, 1 << 62, 16, 64), (8, 2, 1, 1, 1 << 62, 64),
+                (8, 2, 1, 1, 16, 20), (1 << 62, 2, 1, 1, 16, 64)):
+        for n in (None, 5, 1 << 62):
+            with pytest.raises(_lib.SapientHipError):
+                ops.paged_attention_workspace(*bad, n_tokens=n)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
