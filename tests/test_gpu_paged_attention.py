@@ -318,3 +318,34 @@ def test_values_that_are_not_finite_stay_in_rows_that_see_them(dev, types):
                 sees[i, 2:] = pos >= at and (not window or pos - at < window)  # heads 2 and 3 read kv head 1
             assert not torch.isfinite(got[sees][:, 5]).any()
             assert torch.equal(got[~sees], clean[~sees])
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches(dev, seed):
+    """Any mix of heads, head_dim, types, pages, lengths, masks and score forms."""
+    r = np.random.default_rng(seed)
+    kv = int(r.integers(1, 6))
+    heads, D = kv * int(r.choice([1, 2, 3, 7, 16, 20])), 8 * int(r.integers(1, 33))
+    dt, ct = TYPES[int(r.integers(len(TYPES)))]
+    chunk = bool(r.integers(2))
+    lens = [int(x) for x in r.integers(0, 260, int(r.integers(1, 6)))]
+    if r.integers(4) == 0:
+        lens[0] = int(r.integers(600, 1500))
+    new = [int(min(n, x)) for n, x in zip(lens, r.integers(0, 150, len(lens)))] if chunk else None
+    if chunk and not sum(new):
+        new[0] = lens[0] = max(1, lens[0])
+    c = Batch(heads, kv, D, lens, new, dt, ct, page=int(r.choice([1, 5, 16, 32, 40, 64, 256])), seed=seed, extra_rows=2 * chunk)
+    m = {}
+    if r.integers(3) == 0:
+        m["softcap"] = float(r.choice([1.0, 20.0]))
+    if r.integers(3) == 0:
+        m["window"] = int(r.integers(1, 300))
+    if r.integers(3) == 0:
+        m["slopes"] = torch.from_numpy(r.uniform(0, 0.5, heads).astype(np.float32))
+    kw = {k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in m.items()}
+    if chunk and r.integers(2):
+        m["prefix"] = [int(x) for x in r.integers(0, 300, len(lens))]
+        kw["prefix_lens"] = torch.tensor(m["prefix"], dtype=torch.int32, device=dev)
+    say("random", seed, heads, kv, D, NAME[dt], NAME[ct], c.page, lens, new, {k: v for k, v in m.items() if k != "slopes"})
+    f = ops.paged_attention_chunk if chunk else ops.paged_attention
+    check(f(*c.to(dev), **kw), c, f"seed {seed}", weights(dt, ct, chunk), **m)

@@ -125,3 +125,48 @@ def test_a_finished_sequence_is_padding(dev):
     pick = torch.tensor([0, 2], device=dev)
     alone = ops.paged_attention(turned[pick].contiguous(), s.kc, s.vc, s.seq_lens[pick].contiguous(), s.table[pick].contiguous())
     assert torch.allclose(out[pick].float(), alone.float(), rtol=2 ** -10, atol=1e-6)
+
+
+def test_threads_on_their_own_streams_and_captured_without_a_workspace(dev):
+    """Calls from several host threads at once, each with its own stream and scratch, and a captured call that allocates its
+    scratch itself: the same bits as one after the other."""
+    import threading
+    servers = [Server(dev, [900 + 7 * i, 5, 130], 2) for i in range(3)]
+    queries = []
+    for s in servers:
+        for t in (s.kc, s.vc):
+            t.normal_()
+        s.seq_lens += torch.tensor([900, 5, 130], dtype=torch.int32, device=dev)
+        queries.append(s.r(3, HEADS, D))
+    call = lambda s, q: ops.paged_attention(q, s.kc, s.vc, s.seq_lens, s.table)
+    want = [call(s, q) for s, q in zip(servers, queries)]
+    torch.cuda.synchronize()
+    got, errors = [None] * 3, []
+
+    def work(i):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(20):
+                    got[i] = call(servers[i], queries[i])
+            st.synchronize()
+        except Exception as e:  # reported below
+            errors.append(repr(e))
+
+    print("case threads", flush=True)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=60)
+    assert not errors and all(torch.equal(g, w) for g, w in zip(got, want)), errors
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(want[0])
+    with torch.cuda.graph(graph):
+        ops.paged_attention(queries[0], servers[0].kc, servers[0].vc, servers[0].seq_lens, servers[0].table, out=out)
+    for n in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        print("case replay", n, flush=True)
+        assert torch.equal(out, want[0])
